@@ -38,6 +38,11 @@ extern "C" {
 #define PHONLP_ERR_LAUNCH (-3)      /* HIP reported a launch error */
 #define PHONLP_ERR_UNSUPPORTED (-4) /* size beyond what the kernels support (e.g. T > 64) */
 
+/* element types of the entry points that take more than fp32 */
+#define PHONLP_F32 0
+#define PHONLP_BF16 1
+#define PHONLP_F16 2
+
 /* per-sentence status written by phonlp_mst_one_root */
 #define PHONLP_MST_OK 0
 #define PHONLP_MST_NO_FINITE_TREE 1 /* ref chuliu_edmonds.py:162-168: the reference asserts here */
@@ -503,6 +508,48 @@ int phonlp_pos_loss(const float *upos_logits, const int32_t *gold_upos, const in
  * count: DEVICE pointer to the number of counted words (loss + 2 of phonlp_pos_loss), read by the kernel. */
 int phonlp_pos_loss_grad(const float *upos_logits, const int32_t *gold_upos, const int32_t *sentlens,
                          const float *count, int B, int L, int U, int ignore_index, float *d_logits, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit dense layer and embedding rows, for training beside (and inference below) the fp32-grade layers above; no counterpart
+ * in the reference, whose layers are fp32.  Element types: PHONLP_F32 / _BF16 / _F16.
+ *
+ * An e4m3 image of a matrix x [rows, K] (8-bit floating point, OCP e4m3: 4 exponent and 3 mantissa bits, largest 448) has one
+ * power-of-two scale per row and block of 128 columns: with a = the block's largest finite magnitude, e = the smallest integer
+ * >= -126 with a <= 448 * 2^e, code = e4m3(x * 2^-e) rounded to nearest even (at most 240 for e = 120: no value passes fp32's
+ * largest); infinities and NaN become the NaN code.  An entry is off by at most 2^-4 of itself, or by 2^(e-10) below 2^(e-6).
+ *   codes      [rows, phonlp_e4m3_kp(K)] bytes, K rounded up to 128, zero behind K; 16-byte aligned
+ *   exponents  [rows, phonlp_e4m3_kb(K)] bytes, e + 127; the number of blocks rounded up to 4, 127 behind; 4-byte aligned
+ * phonlp_e4m3_rows makes an image (x: row pitch ldx >= K elements, any alignment of its type), phonlp_e4m3_values gives the
+ * values back, out [rows, K]; 16-bit types saturate at their largest.  K <= 2^22. */
+int phonlp_e4m3_kp(int K);
+int phonlp_e4m3_kb(int K);
+int phonlp_e4m3_rows(const void *x, int type, long ldx, int rows, int K, void *codes, uint8_t *exponents, void *stream);
+int phonlp_e4m3_values(const void *codes, const uint8_t *exponents, int rows, int K, int type, void *out, void *stream);
+
+/* Y[M,N] = act(X^ . W^^T + bias[N]) with X^, W^ the values of two images with the same K; fp32 sums, Y in `type`, row pitch N.
+ * bias may be NULL.  relu: max(., 0), NaN kept.  bits: NULL, or [M, ceil(N / 32)] words with bit n % 32 of word n / 32 set where
+ * Y[m][n] > 0 before its rounding to `type` (zero behind N) -- what the backward needs of a ReLU layer's output. */
+int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents,
+                       const float *bias, void *y, int type, uint32_t *bits, int M, int N, int K, int relu, void *stream);
+
+/* Backward of that layer from its 8-bit checkpoint: dY [M,N] in `type` (row pitch lddy), bits as above (NULL: no ReLU), the images
+ * of the layer's input and weight ->  dZ = dY where the bit is set, dX [M,K] = dZ . W^ in `type`, dW [N,K] = dZ^T . X^ and
+ * db [N] = column sums of dZ in fp32.  Any of dX / dW / db may be NULL.  Products are exact (dZ in up to three bf16 pieces), sums
+ * fp32 in a fixed order.  M <= 2^24, N and K <= 2^21. */
+size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int type);
+int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, const uint32_t *bits, const void *x_codes,
+                                const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents, int M, int N, int K,
+                                void *dx, float *dw, float *db, void *ws, size_t ws_bytes, void *stream);
+
+/* out[n] = scale * table[tokens[n]], n < N; table [V,E] (row pitch ld), tokens int32 or int64, out [N,E] of the table's type.
+ * A token outside [0, V) gives a row of zeros.  Its gradient: d_table[v] = scale * sum of d_out[n] over the n with tokens[n] = v,
+ * every row of d_table [V,E] written (zeros where no token points), of d_out's type or fp32; fp32 sums in an order that depends
+ * on the tokens alone.  N <= 2^30, E <= 2^22. */
+int phonlp_embedding_rows(const void *table, int type, long ld, const void *tokens, int tokens_are_int64, int N, int V, int E,
+                          float scale, void *out, void *stream);
+size_t phonlp_embedding_rows_grad_ws_bytes(int N, int E);
+int phonlp_embedding_rows_grad(const void *d_out, int type, long ld, const void *tokens, int tokens_are_int64, int N, int V,
+                               int E, float scale, void *d_table, int table_type, void *ws, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------------
  * Per-kernel timing (no counterpart in the reference, which has no profiling: SURVEY.md section 5).

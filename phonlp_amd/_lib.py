@@ -6,7 +6,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libphonlp_heads.so")
 
-_i, _z, _p, _f = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float
+_i, _z, _p, _f, _l = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float, ctypes.c_long
 
 # name -> (restype, argtypes); mirrors include/phonlp_heads.h declaration by declaration
 SIGNATURES = {
@@ -83,6 +83,16 @@ SIGNATURES = {
     "phonlp_pos_loss_ws_bytes": (_z, [_i, _i]),
     "phonlp_pos_loss": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p, _z, _p]),
     "phonlp_pos_loss_grad": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "phonlp_e4m3_kp": (_i, [_i]),
+    "phonlp_e4m3_kb": (_i, [_i]),
+    "phonlp_e4m3_rows": (_i, [_p, _i, _l, _i, _i, _p, _p, _p]),
+    "phonlp_e4m3_values": (_i, [_p, _p, _i, _i, _i, _p, _p]),
+    "phonlp_linear_e4m3": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _p]),
+    "phonlp_linear_e4m3_backward_ws_bytes": (_z, [_i, _i, _i, _i]),
+    "phonlp_linear_e4m3_backward": (_i, [_p, _i, _l, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p, _p, _z, _p]),
+    "phonlp_embedding_rows": (_i, [_p, _i, _l, _p, _i, _i, _i, _i, _f, _p, _p]),
+    "phonlp_embedding_rows_grad_ws_bytes": (_z, [_i, _i]),
+    "phonlp_embedding_rows_grad": (_i, [_p, _i, _l, _p, _i, _i, _i, _i, _f, _p, _i, _p, _z, _p]),
     "phonlp_profile_begin": (_i, [_i]),
     "phonlp_profile_end": (_i, [_p, _p, _i]),
     "phonlp_profile_only": (_i, [ctypes.c_char_p]),

@@ -1,0 +1,438 @@
+// Embedding lookup with scaling, out[n] = scale * table[token_n], and its gradient by sorted tokens,
+// d_table[v] = scale * sum over the n with token_n = v of d_out[n]  (a token outside [0, V): a zero row, no gradient).
+//
+// The gradient sorts (token, n) stably, so that a token's rows stand together in ascending n; one wave sums the rows of a fixed
+// number of sorted places and writes the runs of equal tokens that lie inside, runs that reach over a border leave fp32 shares
+// that a second launch adds in order.  No float atomics: the result does not depend on the launch, and a token that holds a large
+// share of all places is summed by as many waves as its places fill.  Both directions are bound by memory.
+#include "e4m3.h"
+
+namespace phonlp {
+
+template <class I>
+__device__ __forceinline__ int token_key(const I *tokens, long n, int V) {  // V: no row
+    const I t = tokens[n];
+    return t >= 0 && t < (I)V ? (int)t : V;
+}
+
+template <class T, class I>
+__global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, long ld, const I *tokens, int N, int V, int E, float scale,
+                                                             T *out) {
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 4;
+    typedef typename Vec<T, VEC>::type Vt;
+    const int per_row = (E + VEC - 1) / VEC;
+    const long total = (long)N * per_row, step = (long)gridDim.x * 256;
+    for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < total; g += step * UNROLL) {
+        Vt v[UNROLL];
+        long at[UNROLL];
+        int left[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const long it = g + u * step;
+            left[u] = 0;
+            if (it >= total) continue;
+            const long n = total < (1L << 31) ? (long)((unsigned)it / (unsigned)per_row) : it / per_row;
+            const int c = (int)(it - n * per_row) * VEC, key = token_key(tokens, n, V);
+            at[u] = n * E + c;
+            left[u] = min(E - c, VEC);
+            const T *p = table + key * ld + c;
+            if (key < V && left[u] == VEC) {
+                v[u] = *reinterpret_cast<const Vt *>(p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = key < V && i < left[u] ? p[i] : (T)0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[u][i] = (T)((float)v[u][i] * scale);
+            if (left[u] == VEC) {
+                *reinterpret_cast<Vt *>(out + at[u]) = v[u];
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (i < left[u]) out[at[u] + i] = v[u][i];
+            }
+        }
+    }
+}
+
+// ---- sorting, few tokens: a token's place is the number of (token, n) pairs before its own.  N^2 comparisons of which each is two
+// instructions, one launch.  A workgroup places 32 tokens, eight threads count an eighth of the others each.
+template <class I>
+__global__ __launch_bounds__(256) void embedding_place_kernel(const I *tokens, int N, int V, int *order, int *sorted) {
+    __shared__ int keys[2048];
+    __shared__ int counts[8][32];
+    const int own = threadIdx.x & 31, part = threadIdx.x >> 5, n = blockIdx.x * 32 + own;
+    const int key = n < N ? token_key(tokens, n, V) : 0;
+    int count = 0;
+    for (int base = 0; base < N; base += 2048) {
+        const int here = min(2048, N - base);
+        __syncthreads();
+        for (int i = threadIdx.x; i < here; i += 256) keys[i] = token_key(tokens, base + i, V);
+        __syncthreads();
+        const int lo = part * 256, hi = min(lo + 256, here);
+        // before n equal tokens count too
+        for (int i = lo; i < hi; ++i) count += keys[i] < key + (base + i < n ? 1 : 0);
+    }
+    counts[part][own] = count;
+    __syncthreads();
+    if (part == 0 && n < N) {
+        int place = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) place += counts[i][own];
+        order[place] = n;
+        sorted[place] = key;
+    }
+}
+
+// ---- sorting, many tokens: stable radix passes of eight bits, tiles of 4096 pairs.
+constexpr int kSortTile = 4096;
+
+template <class I>
+__device__ __forceinline__ int sort_key(const I *tokens, const int *keys, long n, int V) {
+    return keys ? keys[n] : token_key(tokens, n, V);
+}
+
+// counts[digit][tile]
+template <class I>
+__global__ __launch_bounds__(256) void embedding_count_kernel(const I *tokens, const int *keys, int N, int V, int shift, int tiles, int *counts) {
+    __shared__ int bins[256];
+    bins[threadIdx.x] = 0;
+    __syncthreads();
+    const long base = (long)blockIdx.x * kSortTile;
+    for (int i = threadIdx.x; i < kSortTile && base + i < N; i += 256) atomicAdd(&bins[sort_key(tokens, keys, base + i, V) >> shift & 255], 1);
+    __syncthreads();
+    counts[(long)threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
+}
+
+// counts -> the number of pairs before (digit, tile), in place; one workgroup
+__global__ __launch_bounds__(1024) void embedding_scan_kernel(int *counts, int total) {
+    __shared__ int waves[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int carry = 0;
+    for (int base = 0; base < total; base += 1024) {
+        const int i = base + threadIdx.x;
+        const int v = i < total ? counts[i] : 0;
+        int s = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(s, d);
+            if (lane >= d) s += o;
+        }
+        if (lane == 63) waves[wave] = s;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? waves[w] : 0;
+            all += waves[w];
+        }
+        if (i < total) counts[i] = carry + before + s - v;
+        carry += all;
+        __syncthreads();
+    }
+}
+
+template <class I>
+__global__ __launch_bounds__(256) void embedding_scatter_kernel(const I *tokens, const int *keys, const int *index, int N, int V, int shift,
+                                                                int tiles, const int *before, int *keys_out, int *index_out) {
+    __shared__ int at[4][256];  // the next place of each wave's pairs of a digit
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long base = (long)blockIdx.x * kSortTile + wave * (kSortTile / 4);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) at[w][threadIdx.x] = 0;
+    __syncthreads();
+    for (int r = 0; r < kSortTile / 4; r += 64) {
+        const long n = base + r + lane;
+        if (n < N) atomicAdd(&at[wave][sort_key(tokens, keys, n, V) >> shift & 255], 1);
+    }
+    __syncthreads();
+    int place = before[(long)threadIdx.x * tiles + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int c = at[w][threadIdx.x];
+        at[w][threadIdx.x] = place;
+        place += c;
+    }
+    __syncthreads();
+    for (int r = 0; r < kSortTile / 4; r += 64) {
+        const long n = base + r + lane;
+        const bool in = n < N;
+        const int key = in ? sort_key(tokens, keys, n, V) : 0, digit = key >> shift & 255;
+        // the lanes that hold a pair of the same digit
+        unsigned long long same = __ballot(in);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const unsigned long long set = __ballot(digit >> b & 1);
+            same &= digit >> b & 1 ? set : ~set;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        int first = 0;
+        if (in) first = at[wave][digit];
+        __builtin_amdgcn_wave_barrier();
+        if (in) {
+            keys_out[first + rank] = key;
+            index_out[first + rank] = index ? index[n] : (int)n;
+            if (rank == 0) at[wave][digit] = first + __popcll(same);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- sums
+// The first place >= lo whose token is >= key.
+__device__ __forceinline__ int lower_bound(const int *sorted, int lo, int hi, int key) {
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sorted[mid] < key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <class T, int VEC>
+__device__ __forceinline__ void load_row(const T *p, int left, float (&v)[VEC]) {
+    typedef typename Vec<T, VEC>::type Vt;
+    if (left >= VEC) {
+        const Vt t = *reinterpret_cast<const Vt *>(p);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = (float)t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+    }
+}
+template <class TO, int VEC>
+__device__ __forceinline__ void store_row(TO *p, int left, const float (&v)[VEC], float scale) {
+    typedef typename Vec<TO, VEC>::type Vt;
+    if (left >= VEC) {
+        Vt t;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) t[i] = (TO)(v[i] * scale);
+        *reinterpret_cast<Vt *>(p) = t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < left) p[i] = (TO)(v[i] * scale);
+    }
+}
+
+struct SumArgs {
+    const void *d_out;
+    void *d_table;
+    float *shares;  // [chunks][2][E]: the sum of a chunk's first run that began before it, of its last run that goes on behind it
+    const int *order, *sorted;
+    long ld;
+    int N, V, E, R, chunks, sum_blocks;
+    float scale;
+};
+
+// blockIdx.y: a slab of 64 * VEC columns.  blockIdx.x < sum_blocks: a wave per chunk of R sorted places; behind them: a wave per 64
+// rows of the table, which writes zeros where no token points.
+template <class T, class TO>
+__global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 8;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = (blockIdx.y * 64 + lane) * VEC, left = a.E - col;
+    TO *table = (TO *)a.d_table;
+    if ((int)blockIdx.x >= a.sum_blocks) {
+        const long row0 = ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 64;
+        const long row = row0 + lane;
+        bool empty = false;
+        if (row < a.V) {
+            const int at = lower_bound(a.sorted, 0, a.N, (int)row);
+            empty = at == a.N || a.sorted[at] != (int)row;
+        }
+        unsigned long long rows = __ballot(empty);
+        const float zero[VEC] = {};
+        while (rows) {
+            const int r = __ffsll(rows) - 1;
+            rows &= rows - 1;
+            if (left > 0) store_row<TO, VEC>(table + (row0 + r) * a.E + col, left, zero, 0.f);
+        }
+        return;
+    }
+    const int chunk = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
+    if (chunk >= a.chunks) return;
+    const int first = chunk * a.R, last = min(first + a.R, a.N);
+    const T *d = (const T *)a.d_out;
+    const bool joined = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
+    bool head = joined;
+    float s[VEC] = {};
+    for (int p = first; p < last; p += UNROLL) {
+        float v[UNROLL][VEC];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int q = min(p + u, last - 1);
+            if (left > 0) load_row<T, VEC>(d + (long)a.order[q] * a.ld + col, left, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int q = p + u;
+            if (q >= last) break;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s[i] += v[u][i];
+            const int key = a.sorted[q];
+            const bool ends = q + 1 >= a.N || a.sorted[q + 1] != key;
+            if (!ends && q + 1 < last) continue;
+            if (left > 0 && key < a.V) {
+                if (ends && !head) store_row<TO, VEC>(table + (long)key * a.E + col, left, s, a.scale);
+                else store_row<float, VEC>(a.shares + ((long)chunk * 2 + (head ? 0 : 1)) * a.E + col, left, s, 1.f);
+            }
+            head = false;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+        }
+    }
+}
+
+// A wave per chunk whose last run begins in it and goes on behind it: the run's shares, in order.
+template <class T, class TO>
+__global__ __launch_bounds__(256) void embedding_join_kernel(SumArgs a) {
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 8;
+    const int lane = threadIdx.x & 63, col = (blockIdx.y * 64 + lane) * VEC, left = a.E - col;
+    const int chunk = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (chunk >= a.chunks - 1) return;
+    const int first = chunk * a.R, next = first + a.R, key = a.sorted[next - 1];
+    if (key >= a.V || a.sorted[next] != key) return;
+    if (a.sorted[first] == key && first > 0 && a.sorted[first - 1] == key) return;  // began before this chunk
+    const int end = lower_bound(a.sorted, next, a.N, key + 1);
+    const int last = (end - 1) / a.R;  // the chunk of the run's last place
+    if (left <= 0) return;
+    float s[VEC];
+    load_row<float, VEC>(a.shares + ((long)chunk * 2 + 1) * a.E + col, left, s);
+    for (int c = chunk + 1; c <= last; c += UNROLL) {
+        float v[UNROLL][VEC];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) load_row<float, VEC>(a.shares + (long)min(c + u, last) * 2 * a.E + col, left, v[u]);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (c + u <= last) s[i] += v[u][i];
+    }
+    store_row<TO, VEC>((TO *)a.d_table + (long)key * a.E + col, left, s, a.scale);
+}
+
+constexpr int kPlaceMost = 16384;
+static int sum_places(int N) {  // sorted places of one wave: few enough to fill the chip, few enough chunks to join
+    int R = ceil_div(ceil_div(N, 2048), 32) * 32;
+    return R;
+}
+struct EmbeddingPlan {
+    int R, chunks, tiles;
+    size_t pairs, shares, counts, total;
+};
+static EmbeddingPlan plan_embedding(int N, int E) {
+    EmbeddingPlan p;
+    p.R = sum_places(N);
+    p.chunks = ceil_div(N, p.R);
+    p.tiles = ceil_div(N, kSortTile);
+    p.pairs = align_up((size_t)N * 4, 256);
+    p.shares = align_up((size_t)p.chunks * 2 * E * 4, 256);
+    const bool radix = N > kPlaceMost;
+    p.counts = radix ? align_up((size_t)p.tiles * 256 * 4, 256) : 0;
+    p.total = p.pairs * (radix ? 4 : 2) + p.shares + p.counts;
+    return p;
+}
+
+template <class I>
+static int sort_tokens(const I *tokens, int N, int V, const EmbeddingPlan &pl, char *ws, int **order, int **sorted, hipStream_t st) {
+    ProfScope ps("embedding_sort", st);
+    int *k[2] = {(int *)ws, (int *)(ws + pl.pairs)};
+    if (N <= kPlaceMost) {
+        hipLaunchKernelGGL((embedding_place_kernel<I>), dim3(ceil_div(N, 32)), dim3(256), 0, st, tokens, N, V, k[0], k[1]);
+        *order = k[0];
+        *sorted = k[1];
+        return check_launch("embedding_place_kernel");
+    }
+    int *keys[2] = {k[0], k[1]}, *index[2] = {(int *)(ws + 2 * pl.pairs), (int *)(ws + 3 * pl.pairs)};
+    int *counts = (int *)(ws + 4 * pl.pairs + pl.shares);
+    const int *from_keys = nullptr, *from_index = nullptr;
+    int now = 0;
+    for (int shift = 0; shift == 0 || (shift < 31 && (V >> shift) > 0); shift += 8, now ^= 1) {  // keys 0 .. V
+        hipLaunchKernelGGL((embedding_count_kernel<I>), dim3(pl.tiles), dim3(256), 0, st, tokens, from_keys, N, V, shift, pl.tiles, counts);
+        hipLaunchKernelGGL(embedding_scan_kernel, dim3(1), dim3(1024), 0, st, counts, pl.tiles * 256);
+        hipLaunchKernelGGL((embedding_scatter_kernel<I>), dim3(pl.tiles), dim3(256), 0, st, tokens, from_keys, from_index, N, V, shift,
+                           pl.tiles, counts, keys[now], index[now]);
+        const int rc = check_launch("embedding_scatter_kernel");
+        if (rc) return rc;
+        from_keys = keys[now];
+        from_index = index[now];
+    }
+    *sorted = keys[now ^ 1];
+    *order = index[now ^ 1];
+    return PHONLP_OK;
+}
+
+template <class T, class TO>
+static int sum_rows(SumArgs a, hipStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int slabs = ceil_div(a.E, 64 * VEC);
+    a.sum_blocks = ceil_div(a.chunks, 4);
+    {
+        ProfScope ps("embedding_sum", st);
+        hipLaunchKernelGGL((embedding_sum_kernel<T, TO>), dim3(a.sum_blocks + ceil_div(a.V, 256), slabs), dim3(256), 0, st, a);
+        const int rc = check_launch("embedding_sum_kernel");
+        if (rc || a.chunks == 1) return rc;
+    }
+    ProfScope ps("embedding_join", st);
+    hipLaunchKernelGGL((embedding_join_kernel<T, TO>), dim3(ceil_div(a.chunks - 1, 4), slabs), dim3(256), 0, st, a);
+    return check_launch("embedding_join_kernel");
+}
+
+}  // namespace phonlp
+
+using namespace phonlp;
+
+extern "C" int phonlp_embedding_rows(const void *table, int type, long ld, const void *tokens, int tokens_are_int64, int N, int V, int E,
+                                     float scale, void *out, void *stream) {
+    if (!table || !tokens || !out || !type_ok(type) || N <= 0 || V <= 0 || E <= 0 || ld < E || V == 0x7FFFFFFF)
+        return fail(PHONLP_ERR_SHAPE, "embedding_rows: bad argument");
+    if ((uintptr_t)table % type_bytes(type) || (uintptr_t)out % type_bytes(type) || (uintptr_t)tokens % (tokens_are_int64 ? 8 : 4))
+        return fail(PHONLP_ERR_SHAPE, "embedding_rows: table, tokens and out must have their types' alignment");
+    hipStream_t st = as_stream(stream);
+    ProfScope ps("embedding_rows", st);
+    return with_type(type, [&](auto t) {
+        using T = decltype(t);
+        constexpr int VEC = 16 / sizeof(T);
+        const long blocks = ((long)N * ceil_div(E, VEC) + 255) / 256;
+        const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+        if (tokens_are_int64)
+            hipLaunchKernelGGL((embedding_rows_kernel<T, long>), grid, dim3(256), 0, st, (const T *)table, ld, (const long *)tokens, N, V, E,
+                               scale, (T *)out);
+        else
+            hipLaunchKernelGGL((embedding_rows_kernel<T, int>), grid, dim3(256), 0, st, (const T *)table, ld, (const int *)tokens, N, V, E,
+                               scale, (T *)out);
+        return check_launch("embedding_rows_kernel");
+    });
+}
+
+extern "C" size_t phonlp_embedding_rows_grad_ws_bytes(int N, int E) {
+    return N > 0 && N <= (1 << 30) && E > 0 && E <= (1 << 22) ? plan_embedding(N, E).total : 0;
+}
+
+extern "C" int phonlp_embedding_rows_grad(const void *d_out, int type, long ld, const void *tokens, int tokens_are_int64, int N, int V,
+                                          int E, float scale, void *d_table, int table_type, void *ws, size_t ws_bytes, void *stream) {
+    if (!d_out || !tokens || !d_table || !type_ok(type) || N <= 0 || N > (1 << 30) || V <= 0 || V == 0x7FFFFFFF || E <= 0 ||
+        E > (1 << 22) || ld < E || (table_type != type && table_type != PHONLP_F32))
+        return fail(PHONLP_ERR_SHAPE, "embedding_rows_grad: bad argument (d_table is of d_out's type or fp32)");
+    if ((uintptr_t)d_out % type_bytes(type) || (uintptr_t)d_table % type_bytes(table_type) || (uintptr_t)tokens % (tokens_are_int64 ? 8 : 4))
+        return fail(PHONLP_ERR_SHAPE, "embedding_rows_grad: d_out, tokens and d_table must have their types' alignment");
+    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < phonlp_embedding_rows_grad_ws_bytes(N, E))
+        return fail(PHONLP_ERR_WORKSPACE, "embedding_rows_grad: workspace too small or not 16-byte aligned");
+    hipStream_t st = as_stream(stream);
+    const EmbeddingPlan pl = plan_embedding(N, E);
+    const bool radix = N > kPlaceMost;
+    int *order, *sorted;
+    const int rc = tokens_are_int64 ? sort_tokens((const long *)tokens, N, V, pl, (char *)ws, &order, &sorted, st)
+                                    : sort_tokens((const int *)tokens, N, V, pl, (char *)ws, &order, &sorted, st);
+    if (rc) return rc;
+    SumArgs a = {d_out, d_table, (float *)((char *)ws + pl.pairs * (radix ? 4 : 2)), order, sorted, ld, N, V, E, pl.R, pl.chunks, 0, scale};
+    return with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (table_type == PHONLP_F32) return sum_rows<T, float>(a, st);
+        return sum_rows<T, T>(a, st);
+    });
+}

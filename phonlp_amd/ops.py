@@ -951,6 +951,203 @@ def pos_head_split(enc: Tensor, sentlens: Tensor, Whid: Tensor, bhid: Tensor, Wc
 # what the op itself allocates -- same shapes and dtypes; tests/test_fake_ops.py checks them against the real outputs.
 _I32, _I64, _U8 = torch.int32, torch.int64, torch.uint8
 
+# ---------------------------------------------------------------- 8-bit dense layer and embedding rows (include/phonlp_heads.h)
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_E4M3 = torch.float8_e4m3fn
+
+
+def _run(device, name, *args):
+    """One C-ABI call on `device`'s current stream (the tensors' device need not be the current one)."""
+    f = getattr(lib(), name)
+    if _raw_device is not None and device.index == _raw_device():
+        rc = f(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        check(rc, name)
+
+
+def _rows_of(t: Tensor, name: str):
+    """A 2-d device tensor of fp32 / bf16 / fp16 rows with unit column stride -> (type code, row pitch)."""
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: expected dtype float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a ROCm device tensor (phonlp_amd has no CPU path)")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected 2 dimensions, got {t.dim()}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        raise ValueError(f"{name}: expected rows of unit column stride that do not overlap (pass .contiguous())")
+    return code, max(t.stride(0), cols) if rows > 1 else cols
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: expected a tensor on {device}, got {t.device}")
+
+
+def e4m3_kp(K: int) -> int:
+    """Codes per row of an e4m3 image: K rounded up to 128."""
+    return -(-K // 128) * 128
+
+
+def e4m3_kb(K: int) -> int:
+    """Exponents per row of an e4m3 image: the number of blocks of 128 rounded up to 4."""
+    return -(-K // 512) * 4
+
+
+def _image_of(codes: Tensor, exponents: Tensor, K: int, name: str) -> int:
+    """Checks an e4m3 image of [rows, K]; -> rows."""
+    if codes.dtype != _E4M3 or exponents.dtype != torch.uint8:
+        raise ValueError(f"{name}: expected float8_e4m3fn codes and uint8 exponents, got {codes.dtype} and {exponents.dtype}")
+    if not codes.is_cuda:
+        raise ValueError(f"{name}: expected a ROCm device tensor (phonlp_amd has no CPU path)")
+    if K < 1 or codes.dim() != 2 or codes.shape[1] != e4m3_kp(K) or tuple(exponents.shape) != (codes.shape[0], e4m3_kb(K)):
+        raise ValueError(f"{name}: expected codes [rows, {e4m3_kp(K)}] and exponents [rows, {e4m3_kb(K)}] for K = {K}, "
+                         f"got {tuple(codes.shape)} and {tuple(exponents.shape)}")
+    if not (codes.is_contiguous() and exponents.is_contiguous()):
+        raise ValueError(f"{name}: expected contiguous tensors")
+    if exponents.device != codes.device:
+        raise ValueError(f"{name}: codes and exponents are on different devices")
+    return codes.shape[0]
+
+
+def e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """x [rows, K] fp32 / bf16 / fp16 (row stride free, unit column stride) -> its e4m3 image: codes float8_e4m3fn
+    [rows, e4m3_kp(K)], exponents uint8 [rows, e4m3_kb(K)] (one power-of-two scale per row and block of 128 columns; infinities and
+    NaN become NaN).  The operand form of linear_e4m3, and a layer input's 8-bit checkpoint for linear_e4m3_backward."""
+    code, ld = _rows_of(x, "x")
+    rows, K = x.shape
+    if K == 0:
+        raise ValueError("e4m3_rows: x has no columns")
+    dev = x.device
+    codes = torch.empty((rows, e4m3_kp(K)), dtype=_E4M3, device=dev)
+    exponents = torch.empty((rows, e4m3_kb(K)), dtype=torch.uint8, device=dev)
+    if rows:
+        _run(dev, "phonlp_e4m3_rows", x.data_ptr(), code, ld, rows, K, codes.data_ptr(), exponents.data_ptr())
+    return codes, exponents
+
+
+def e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype = torch.float32) -> Tensor:
+    """The values [rows, K] that an e4m3 image stands for: exact in fp32 and bf16, 16-bit types saturate at their largest."""
+    rows = _image_of(codes, exponents, K, "codes")
+    if dtype not in _TYPES:
+        raise ValueError(f"e4m3_values: dtype must be float32, bfloat16 or float16, got {dtype}")
+    dev = codes.device
+    out = torch.empty((rows, K), dtype=dtype, device=dev)
+    if rows:
+        _run(dev, "phonlp_e4m3_values", codes.data_ptr(), exponents.data_ptr(), rows, K, _TYPES[dtype], out.data_ptr())
+    return out
+
+
+def linear_e4m3(x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponents: Tensor, bias: Optional[Tensor], K: int,
+                relu: bool, dtype: torch.dtype = torch.float32, want_bits: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """y = act(x @ w.T + bias) on the e4m3 images of x [M, K] and w [N, K] (e4m3_rows) -> (y [M, N] in `dtype`, bits).
+    bits (want_bits): int32 [M, ceil(N / 32)], bit n % 32 of word n / 32 set where y > 0 -- what linear_e4m3_backward needs of a
+    ReLU layer; else None."""
+    M = _image_of(x_codes, x_exponents, K, "x_codes")
+    N = _image_of(w_codes, w_exponents, K, "w_codes")
+    dev = x_codes.device
+    _same_device(dev, w_codes=w_codes, bias=bias)
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+        raise ValueError(f"bias: expected a contiguous float32 tensor [{N}], got {bias.dtype} {tuple(bias.shape)}")
+    if dtype not in _TYPES:
+        raise ValueError(f"linear_e4m3: dtype must be float32, bfloat16 or float16, got {dtype}")
+    y = torch.empty((M, N), dtype=dtype, device=dev)
+    bits = torch.empty((M, (N + 31) // 32), dtype=torch.int32, device=dev) if want_bits else None
+    if M and N:
+        _run(dev, "phonlp_linear_e4m3", x_codes.data_ptr(), x_exponents.data_ptr(), w_codes.data_ptr(), w_exponents.data_ptr(),
+             None if bias is None else bias.data_ptr(), y.data_ptr(), _TYPES[dtype], None if bits is None else bits.data_ptr(), M, N, K,
+             int(relu))
+    return y, bits
+
+
+def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor,
+                         w_exponents: Tensor, K: int, need_dX: bool = True, need_dW: bool = True, need_db: bool = True):
+    """Backward of linear_e4m3 from the checkpoint: dY [M, N] fp32 / bf16 / fp16 (row stride free), bits of a ReLU layer (None: no
+    ReLU), the images of the layer's input and weight -> (dX [M, K] of dY's type, dW [N, K] fp32, db [N] fp32), None where not asked
+    for.  The quantisation of x and w counts as the identity."""
+    code, ld = _rows_of(dY, "dY")
+    M = _image_of(x_codes, x_exponents, K, "x_codes")
+    N = _image_of(w_codes, w_exponents, K, "w_codes")
+    dev = dY.device
+    _same_device(dev, x_codes=x_codes, w_codes=w_codes, bits=bits)
+    if tuple(dY.shape) != (M, N):
+        raise ValueError(f"dY: expected [{M}, {N}] by the images, got {tuple(dY.shape)}")
+    if bits is not None and (bits.dtype != torch.int32 or tuple(bits.shape) != (M, (N + 31) // 32) or not bits.is_contiguous()):
+        raise ValueError(f"bits: expected a contiguous int32 tensor [{M}, {(N + 31) // 32}], got {bits.dtype} {tuple(bits.shape)}")
+    if M == 0 or N == 0:  # empty sums
+        zeros = lambda *shape, t: torch.zeros(shape, dtype=t, device=dev)
+        return (zeros(M, K, t=dY.dtype) if need_dX else None, zeros(N, K, t=torch.float32) if need_dW else None,
+                zeros(N, t=torch.float32) if need_db else None)
+    dX = torch.empty((M, K), dtype=dY.dtype, device=dev) if need_dX else None
+    dW = torch.empty((N, K), dtype=torch.float32, device=dev) if need_dW else None
+    db = torch.empty((N,), dtype=torch.float32, device=dev) if need_db else None
+    if not (need_dX or need_dW or need_db):
+        return None, None, None
+    nb = lib().phonlp_linear_e4m3_backward_ws_bytes(M, N, K, code)
+    ws = _ws(nb, dev)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    _run(dev, "phonlp_linear_e4m3_backward", dY.data_ptr(), code, ld, ptr(bits), x_codes.data_ptr(), x_exponents.data_ptr(),
+         w_codes.data_ptr(), w_exponents.data_ptr(), M, N, K, ptr(dX), ptr(dW), ptr(db), ws.data_ptr(), max(nb, 256))
+    return dX, dW, db
+
+
+def _tokens_of(tokens: Tensor, device) -> int:
+    if tokens.dtype not in (torch.int32, torch.int64) or not tokens.is_contiguous():
+        raise ValueError(f"tokens: expected a contiguous int32 or int64 tensor, got {tokens.dtype}")
+    _same_device(device, tokens=tokens)
+    return tokens.numel()
+
+
+def embedding_rows(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
+    """scale * table[tokens]: table [V, E] fp32 / bf16 / fp16 (row stride free), tokens int32 / int64 of any shape -> [*tokens.shape,
+    E] of the table's type.  A token outside [0, V) gives a row of zeros."""
+    code, ld = _rows_of(table, "table")
+    N = _tokens_of(tokens, table.device)
+    V, E = table.shape
+    out = torch.empty((*tokens.shape, E), dtype=table.dtype, device=table.device)
+    if V == 0:
+        return out.zero_()
+    if N and E:
+        _run(table.device, "phonlp_embedding_rows", table.data_ptr(), code, ld, tokens.data_ptr(), int(tokens.dtype == torch.int64), N,
+             V, E, float(scale), out.data_ptr())
+    return out
+
+
+def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> Tensor:
+    """Gradient of embedding_rows for its table: d_out [*tokens.shape, E] -> d_table [V, E], d_table[v] = scale * the sum of the rows
+    whose token is v (zeros where there are none), of d_out's type or `dtype` = float32.  Sums in fp32, by sorted tokens: the same
+    tokens give the same bits."""
+    if d_out.dim() < 1 or tuple(d_out.shape[:-1]) != tuple(tokens.shape):
+        raise ValueError(f"d_out: expected [*{tuple(tokens.shape)}, E], got {tuple(d_out.shape)}")
+    E = d_out.shape[-1]
+    if d_out.dim() != 2:
+        if not d_out.is_contiguous():
+            raise ValueError("d_out: expected a contiguous tensor where tokens is not 1-d")
+        d_out = d_out.view(tokens.numel(), E)
+    code, ld = _rows_of(d_out, "d_out")
+    dev = d_out.device
+    N = _tokens_of(tokens, dev)
+    dtype = d_out.dtype if dtype is None else dtype
+    if dtype not in (d_out.dtype, torch.float32):
+        raise ValueError(f"embedding_rows_grad: dtype must be {d_out.dtype} or float32, got {dtype}")
+    if V < 0:
+        raise ValueError("embedding_rows_grad: V < 0")
+    d_table = torch.empty((V, E), dtype=dtype, device=dev)
+    if N == 0 or V == 0 or E == 0:
+        return d_table.zero_()
+    nb = lib().phonlp_embedding_rows_grad_ws_bytes(N, E)
+    ws = _ws(nb, dev)
+    _run(dev, "phonlp_embedding_rows_grad", d_out.data_ptr(), code, ld, tokens.data_ptr(), int(tokens.dtype == torch.int64), N, V, E,
+         float(scale), d_table.data_ptr(), _TYPES[dtype], ws.data_ptr(), max(nb, 256))
+    return d_table
+
+
+
 
 @linear.register_fake
 def _(x, weight, bias, relu, sentlens, L):
