@@ -159,7 +159,7 @@ def test_linear_bad_values_stay_in_their_rows(dev):
 @pytest.mark.parametrize("relu", [False, True])
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 400, 768), (31, 24, 100), (63, 65, 129), (64, 64, 128), (130, 200, 300), (513, 33, 868),
-                                   (2000, 401, 70), (3001, 64, 64), (40, 2448, 868), (257, 1030, 520), (9000, 130, 260)])
+                                   (2000, 401, 70), (3001, 64, 64), (40, 2448, 868), (257, 1030, 520), (9000, 130, 260), (128, 256, 300), (1920, 384, 129)])
 def test_backward_whole_numbers(dev, dtype, relu, M, N, K):
     """dZ up to 7, values up to 7: sums of up to 9000 products under 2^24, exact; dX is then rounded to dY's type."""
     from phonlp_amd import ops
