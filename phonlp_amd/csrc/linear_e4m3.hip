@@ -21,6 +21,12 @@ struct E4m3Args {
     int M, N, Kp, KB4, num_m, num_n, relu, words;
 };
 
+// LDS image of a tile: row r (128 codes) at r * 128, its 16-byte chunk c at slot c ^ ((r >> 1) & 7): sixteen rows' chunks c lie in
+// sixteen different slots of the 64 banks.
+__device__ __forceinline__ i32x4 tile_chunk(const uint8_t *tile, int r, int c) {
+    return *reinterpret_cast<const i32x4 *>(tile + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+}
+
 // Bias, ReLU, the rounding to T, and the row's bits: acc register r of a lane holds row (r & 3) + 8 (r >> 2) + 4 (lane >> 5),
 // column lane & 31 of a 32 x 32 sub-tile, so one ballot is a 32-column word of two rows.
 template <class T>
@@ -64,7 +70,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_e4m3_kernel(E4m3Args a) {
     extern __shared__ uint8_t lds[];  // [2][TM + TN][128]
     int tm, tn;
     if (!tile_of(blockIdx.x, a.num_m, a.num_n, 8, &tm, &tn)) return;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const int wm = wave / WN, wn = wave % WN;
     const int m0 = tm * TM, n0 = tn * TN;
     const uint8_t *xb = a.x + (long)m0 * a.Kp, *wb = a.w + (long)n0 * a.Kp;
@@ -74,7 +80,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_e4m3_kernel(E4m3Args a) {
     for (int i = 0; i < LOADS; ++i) {  // rows behind the matrix read its last row: their products are not stored
         const int r = (wave + i * NW) * 8 + (lane >> 3);
         const int row = r < TM ? min(r, a.M - 1 - m0) : min(r - TM, a.N - 1 - n0);
-        off[i] = (uint32_t)row * (uint32_t)a.Kp + (((lane & 7) ^ (lane >> 3)) << 4);
+        off[i] = (uint32_t)row * (uint32_t)a.Kp + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
     }
     auto load = [&](int kb, int buf) {
 #pragma unroll
@@ -106,7 +112,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_e4m3_kernel(E4m3Args a) {
 #pragma unroll
             for (int j = 0; j < RB; ++j) sw[j] = *reinterpret_cast<const int *>(we[j] + kb);
         }
-        dma_wait_barrier();  // block kb has landed; everybody is done with the other buffer
+        dma_wait_barrier<0>();  // block kb has landed; everybody is done with the other buffer
         if (kb + 1 < nkb) load(kb + 1, (kb + 1) & 1);
         const uint8_t *A = lds + (kb & 1) * (TM + TN) * 128, *B = A + TM * 128;
         if constexpr (sizeof(T) == 2) {

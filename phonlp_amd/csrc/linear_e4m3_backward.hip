@@ -5,6 +5,8 @@
 // cut into bf16 pieces whose sum is dZ itself -- one for bf16, two for fp16 (11 bits), three for fp32 (24 bits), by truncation, so no
 // piece can round past bf16's largest --, so every product is exact and only the fp32 sums round.  (Values under 2^-126 may lose
 // low bits.)
+#include <type_traits>
+
 #include "e4m3.h"
 #include "tile128.h"
 
@@ -33,42 +35,54 @@ __device__ __forceinline__ void cut(float v, uint16_t (&p)[N]) {
     }
 }
 
-// dY -> the pieces of dZ as rows [P][Mp][Np] (zero behind M and N), and the column sums of 128 rows part[block][n].  A workgroup takes
-// 128 rows x 256 columns, a thread eight columns of every eighth row; the eight threads of a column group add in order.
+// The operands of the two products, in one launch of three kinds of blocks.
+struct BwPrep {
+    const void *dy;
+    long lddy;
+    const uint32_t *bits;
+    uint16_t *planes;  // [P][Mp][Np]
+    float *part;       // column sums of 128 rows, [blocks of rows][N]
+    const uint8_t *codes[2], *exps[2];  // images of x and w
+    __bf16 *wide[2];                    // their values, [rows up to a multiple of 32][Kp]
+    int rows[2], wide_blocks[2];
+    int words, M, N, Mp, Np, Kp, KB4, dz_m, dz_blocks;
+};
+
+// dY -> the pieces of dZ (zero behind M and N) and the column sums.  A workgroup takes 128 rows x 256 columns, a thread eight columns
+// of every eighth row; the eight threads of a column group add in order.
 template <class T>
-__global__ __launch_bounds__(256) void e4m3_bw_dz_kernel(const T *dy, long lddy, const uint32_t *bits, int words, int M, int N, int Mp,
-                                                         int Np, uint16_t *planes, float *part) {
+__device__ __forceinline__ void prep_dz(const BwPrep &a, int bid, float (&sums)[8][256]) {
     constexpr int P = Pieces<T>::N;
     typedef typename Vec<T, 8>::type V;
-    __shared__ float sums[8][256];
-    const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5, n = blockIdx.y * 256 + cg * 8, m0 = blockIdx.x * 128 + rl;
+    const int bm = bid % a.dz_m, bn = bid / a.dz_m;
+    const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5, n = bn * 256 + cg * 8, m0 = bm * 128 + rl;
     float s[8] = {};
-    if (n < Np) {
+    if (n < a.Np) {
 #pragma unroll 4
         for (int it = 0; it < 16; ++it) {
             const int m = m0 + it * 8;
-            if (m >= Mp) break;
+            if (m >= a.Mp) break;
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            if (m < M) {
-                const T *p = dy + m * lddy + n;
-                if (n + 8 <= N) {
+            if (m < a.M) {
+                const T *p = (const T *)a.dy + m * a.lddy + n;
+                if (n + 8 <= a.N) {
                     const V t = *reinterpret_cast<const V *>(p);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (n + i < N) v[i] = (float)p[i];
+                        if (n + i < a.N) v[i] = (float)p[i];
                 }
-                if (bits) {
-                    const uint32_t b = n < N ? bits[(long)m * words + (n >> 5)] >> (n & 31) : 0;
+                if (a.bits) {
+                    const uint32_t b = n < a.N ? a.bits[(long)m * a.words + (n >> 5)] >> (n & 31) : 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = b >> i & 1 ? v[i] : 0.f;
                 }
             }
-            if (planes) {
+            if (a.planes) {
                 uint32_t w[P][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -80,22 +94,55 @@ __global__ __launch_bounds__(256) void e4m3_bw_dz_kernel(const T *dy, long lddy,
                 }
 #pragma unroll
                 for (int q = 0; q < P; ++q)
-                    *reinterpret_cast<uint4 *>(planes + ((long)q * Mp + m) * Np + n) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+                    *reinterpret_cast<uint4 *>(a.planes + ((long)q * a.Mp + m) * a.Np + n) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i] += v[i];
         }
     }
-    if (!part) return;
+    if (!a.part) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sums[rl][cg * 8 + i] = s[i];
     __syncthreads();
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= N) return;
+    const int c = bn * 256 + threadIdx.x;
+    if (c >= a.N) return;
     float t = 0.f;
 #pragma unroll
     for (int r = 0; r < 8; ++r) t += sums[r][threadIdx.x];
-    part[(long)blockIdx.x * N + c] = t;
+    a.part[(long)bm * a.N + c] = t;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void e4m3_bw_prep_kernel(BwPrep a) {
+    __shared__ float sums[8][256];
+    int bid = blockIdx.x;
+    if (bid < a.dz_blocks) return prep_dz<T>(a, bid, sums);
+    bid -= a.dz_blocks;
+    // an image's values in bf16, sixteen codes per thread and turn
+    const int k = bid < a.wide_blocks[0] ? 0 : 1;
+    if (k) bid -= a.wide_blocks[0];
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const int per_row = a.Kp / 16, R = a.rows[k];
+    const long total = (long)((R + 31) / 32 * 32) * per_row, step = a.wide_blocks[k] * 256L;
+    for (long g = bid * 256L + threadIdx.x; g < total; g += step) {
+        const long r = total < (1L << 31) ? (long)((unsigned)g / (unsigned)per_row) : g / per_row;
+        const int c = (int)(g - r * per_row) * 16;
+        i32x4 code = {0, 0, 0, 0};
+        float scale = 1.f;
+        if (r < R) {
+            code = *reinterpret_cast<const i32x4 *>(a.codes[k] + r * a.Kp + c);
+            scale = exp2_biased(a.exps[k][r * a.KB4 + (c >> 7)]);
+        }
+        int w[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[2 * i] = __builtin_bit_cast(int, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[i], scale, false));
+            w[2 * i + 1] = __builtin_bit_cast(int, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[i], scale, true));
+        }
+        i32x4 *o = reinterpret_cast<i32x4 *>(a.wide[k] + r * a.Kp + c);
+        o[0] = i32x4{w[0], w[1], w[2], w[3]};
+        o[1] = i32x4{w[4], w[5], w[6], w[7]};
+    }
 }
 
 // Up to four neighbouring values, rounded to T.
@@ -113,14 +160,13 @@ __device__ __forceinline__ void store_quad(T *p, const f32x4 &v, int left) {
     }
 }
 
-// One of the two products,  C[i][j] = sum_p sum_r A_p(i, r) B[r][j]:  B the values of an image's rows r, columns j; A the pieces of dZ,
-// for dX with i their rows and r their columns, for dW with r their rows and i their columns.
+// One of the two products,  C[i][j] = sum_p sum_r A_p(i, r) B[r][j]:  B the values of an image, bf16 rows r; A the pieces of dZ, for dX
+// with i their rows and r their columns, for dW with r their rows and i their columns.
 struct BwProduct {
-    const uint8_t *a;            // [P][..][pitch bytes]
-    const uint8_t *codes, *exps;  // image of B
-    void *c;                     // [I][J], or fp32 partial sums [S][I][J]
-    long pitch, plane;           // bytes
-    int I, J, R, Kp, KB4, num_i, num_j, per_split, splits, blocks;  // per_split: steps of 64 r
+    const uint8_t *a, *b;  // [P][..][pitch_a bytes], [R up to 32][pitch_b bytes]
+    void *c;               // [I][J], or fp32 partial sums [S][I][J]
+    long pitch_a, plane, pitch_b;
+    int I, J, R, num_i, num_j, per_split, splits, blocks;  // per_split: steps of 32 r
 };
 struct BwArgs {
     BwProduct x, w;
@@ -129,122 +175,114 @@ struct BwArgs {
     int parts, N, db_blocks;
 };
 
-// LDS image of a [64 r][128 columns] bf16 tile: row r at r * 256, its 16-byte chunk c at slot c ^ 4 (r & 3).  A transposing read takes 4
-// rows x 32 bytes per 16 lanes: four different pairs of slots, no bank conflict.
-__device__ __forceinline__ int tr_slot(int r, int c) { return r * 256 + ((c ^ ((r & 3) << 2)) << 4); }
+// LDS images.  Of a tile whose reduction runs along its rows, [i][32 r], 64 bytes a row: chunk c (16 bytes) of row i at slot
+// c ^ ((i >> 2) & 3), so that the chunks c of sixteen rows lie in all 64 banks.  Of a tile whose reduction runs down its rows,
+// [32 r][columns]: chunk c of row r at slot c ^ turn(r); a transposing read takes 4 rows x 32 bytes per 16 lanes, and those of 32
+// lanes (rows 8 apart) lie in all 64 banks.
+__device__ __forceinline__ int turn(int r) { return ((r & 3) << 2) | ((r >> 3 & 1) << 1); }
 
-// The operand of v_mfma_f32_16x16x32_bf16 whose reduction runs down the rows of such a tile: lane l gets column col + (l & 15), rows
-// r0 + 8 (l >> 4) .. + 7.  ds_read_b64_tr_b16: lane i of 16 points at four neighbouring columns of a row (four lanes a row, four rows)
-// and receives four rows of its own column i.
-__device__ __forceinline__ bf16x8 tr_operand(const uint8_t *tile, int r0, int col, int lane) {
+// The operand of v_mfma_f32_16x16x32_bf16 out of such a tile: lane l gets column col + (l & 15), rows 8 (l >> 4) .. + 7.
+// ds_read_b64_tr_b16: lane i of 16 points at four neighbouring columns of a row (four lanes a row, four rows) and receives four rows
+// of its own column i.
+template <int ROW>
+__device__ __forceinline__ bf16x8 tr_operand(const uint8_t *tile, int col, int lane) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 *lds4;
-    const int i = lane & 15, r = r0 + (lane >> 4) * 8 + (i >> 2), c = (col >> 3) + ((i & 3) >> 1);
-    const uint8_t *p = tile + tr_slot(r, c) + (i & 1) * 8;  // the rows four further have the same slot
+    const int i = lane & 15, r = (lane >> 4) * 8 + (i >> 2), c = (col >> 3) + ((i & 3) >> 1);
+    const uint8_t *p = tile + r * ROW + ((c ^ turn(r)) << 4) + (i & 1) * 8;  // the rows four further have the same turn
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * 256));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * ROW));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// 128 x 128 tile, four waves of 64 x 64, steps of 64 r.  A comes by LDS-DMA; B's codes pass through registers, where they take their
-// row's scale (128 columns are one block, so a row has one) and become bf16, eight instructions for sixteen codes.
-template <int P, bool TRANS, class T>
+// The byte offsets, per lane, of kilobyte u of a [32 r][ROW / 2 columns] tile; columns behind the matrix read its last ones.
+template <int ROW>
+__device__ __forceinline__ uint32_t tr_offset(int u, int lane, long pitch, long last) {
+    constexpr int LANES = ROW / 16;
+    const int r = u * (64 / LANES) + lane / LANES, c = (lane % LANES) ^ turn(r);
+    return (uint32_t)r * (uint32_t)pitch + (uint32_t)min((long)c * 16, last);
+}
+
+// Tile of 64 IF x 32 JF, eight waves (4 x 2) of 16 IF x 16 JF, steps of 32 r.  Both operands come by LDS-DMA, three parts (a step and
+// piece) ahead in rings of four; the waits count loads, so that two parts stay in flight.
+template <int P, bool TRANS, int IF, int JF, class T>
 __device__ __forceinline__ void bw_product(const BwProduct &q, int bid, uint8_t *lds) {
-    uint8_t *ta = lds, *tb = lds + 2 * 16384;  // [2][16 KB] each
+    constexpr int TI = IF * 64, TJ = JF * 32, ROWA = TRANS ? TI * 2 : 64, ROWB = JF > 4 ? 512 : 256, SA = TI * 64, SB = 32 * ROWB;
+    constexpr int NA = SA / 8192, NB = SB / 8192;  // loads per wave
+    uint8_t *ta = lds, *tb = lds + 4 * SA;
     int ti, tj;
     const int tiles8 = (q.num_i * q.num_j + 7) / 8 * 8, split = bid / tiles8;
     if (!tile_of(bid - split * tiles8, q.num_i, q.num_j, 8, &ti, &tj)) return;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4, wi = wave >> 1, wj = wave & 1;
-    const int i0 = ti * 128, j0 = tj * 128;
-    const int first = split * q.per_split, last = min(first + q.per_split, ceil_div(q.R, 64)), steps = last - first;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wi = wave >> 1, wj = wave & 1, i0 = ti * TI, j0 = tj * TJ;
+    const int first = split * q.per_split, last = min(first + q.per_split, ceil_div(q.R, 32)), steps = last - first, parts = steps * P;
 
-    uint32_t off[4];
+    uint32_t oa[NA], ob[NB];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int u = wave + k * 4;  // 1 KB of the tile: 8 rows of 128 bytes, or 4 of 256
-        if (TRANS) off[k] = (uint32_t)(u * 4 + (lane >> 4)) * (uint32_t)q.pitch + (((lane & 15) ^ ((lane >> 4) << 2)) << 4);
-        else off[k] = (uint32_t)min(u * 8 + (lane >> 3), q.I - 1 - i0) * (uint32_t)q.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
+    for (int k = 0; k < NA; ++k) {
+        const int u = wave + k * 8, row = u * 16 + (lane >> 2);
+        oa[k] = TRANS ? tr_offset<ROWA>(u, lane, q.pitch_a, q.pitch_a - 16 - i0 * 2L)
+                      : (uint32_t)min(row, q.I - 1 - i0) * (uint32_t)q.pitch_a + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
     }
-    const uint8_t *ab = q.a + (TRANS ? i0 * 2L : i0 * q.pitch);
-    auto load_a = [&](int s, int p, int buf) {
-        const uint8_t *base = ab + p * q.plane + (first + s) * (TRANS ? 64 * q.pitch : 128L);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dma16(base, off[k], ta + buf * 16384 + (wave + k * 4) * 1024);
-    };
-    // codes of rows tid / 8 and 32 + tid / 8, sixteen columns each
-    const int br = tid >> 3, bc = tid & 7;
-    i32x4 code[2];
-    int exps[2];
-    auto load_b = [&](int s) {
+    for (int k = 0; k < NB; ++k) ob[k] = tr_offset<ROWB>(wave + k * 8, lane, q.pitch_b, q.pitch_b - 16 - j0 * 2L);
+    const uint8_t *ab = q.a + (TRANS ? i0 * 2L : i0 * q.pitch_a), *bb = q.b + j0 * 2L;
+    // behind the end the last part is loaded again: the number of loads in flight stays what the waits count
+    auto load = [&](int t, bool b) {
+        const int slot = t & 3, slot_b = t / P & 3;
+        t = min(t, parts - 1);
+        const int s = t / P, p = t - s * P;
+        if (b) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = (first + s) * 64 + h * 32 + br, rr = min(r, q.R - 1);
-            code[h] = *reinterpret_cast<const i32x4 *>(q.codes + (long)rr * q.Kp + j0 + bc * 16);
-            exps[h] = q.exps[(long)rr * q.KB4 + tj];
-            if (r >= q.R) code[h] = i32x4{0, 0, 0, 0};
+            for (int k = 0; k < NB; ++k) dma16(bb + (first + s) * (32 * q.pitch_b), ob[k], tb + slot_b * SB + (wave + k * 8) * 1024);
         }
+#pragma unroll
+        for (int k = 0; k < NA; ++k)
+            dma16(ab + p * q.plane + (first + s) * (TRANS ? 32 * q.pitch_a : 64L), oa[k], ta + slot * SA + (wave + k * 8) * 1024);
     };
-    auto store_b = [&](int buf) {
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    f32x4 acc[IF][JF];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float scale = exp2_biased(exps[h]);
-            int w[8];
+    for (int i = 0; i < IF; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                w[2 * k] = __builtin_bit_cast(int, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[h][k], scale, false));
-                w[2 * k + 1] = __builtin_bit_cast(int, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[h][k], scale, true));
-            }
-            uint8_t *t = tb + buf * 16384;
-            const int r = h * 32 + br;
-            *reinterpret_cast<i32x4 *>(t + tr_slot(r, bc * 2)) = i32x4{w[0], w[1], w[2], w[3]};
-            *reinterpret_cast<i32x4 *>(t + tr_slot(r, bc * 2 + 1)) = i32x4{w[4], w[5], w[6], w[7]};
-        }
-    };
-
-    f32x4 acc[4][4];
+        for (int j = 0; j < JF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    load_a(0, 0, 0);
-    load_b(0);
-    store_b(0);
-    int t = 0;
+    for (int t = 0; t < 3; ++t) load(t, t % P == 0);
     for (int s = 0; s < steps; ++s) {
+        bf16x8 fb[JF];
 #pragma unroll
-        for (int p = 0; p < P; ++p, ++t) {
-            dma_wait_barrier();  // A of this part and B of this step are in LDS; everybody is done with the other buffers
-            if (p + 1 < P) load_a(s, p + 1, (t + 1) & 1);
-            else if (s + 1 < steps) load_a(s + 1, 0, (t + 1) & 1);
-            if (p == 0 && s + 1 < steps) load_b(s + 1);
-            const uint8_t *A = ta + (t & 1) * 16384, *B = tb + (s & 1) * 16384;
+        for (int p = 0; p < P; ++p) {
+            // in flight behind part t: parts t + 1 and t + 2, with B where a step begins
+            constexpr int two = 2 * NA;
+            if (P == 1) dma_wait_barrier<two + 2 * NB>();
+            else if (P == 2 || p > 0) dma_wait_barrier<two + NB>();
+            else dma_wait_barrier<two>();
+            const int t = s * P + p;
+            load(t + 3, (p + 3) % P == 0);
+            const uint8_t *A = ta + (t & 3) * SA, *B = tb + (s & 3) * SB;
+            if (p == 0) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 fa[4], fb[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    fa[i] = TRANS ? tr_operand(A, ks * 32, wi * 64 + i * 16, lane)
-                                  : __builtin_bit_cast(bf16x8, tile_chunk(A, wi * 64 + i * 16 + l16, ks * 4 + g));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) fb[j] = tr_operand(B, ks * 32, wj * 64 + j * 16, lane);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < JF; ++j) fb[j] = tr_operand<ROWB>(B, (wj * JF + j) * 16, lane);
             }
-            if (p + 1 == P && s + 1 < steps) store_b((s + 1) & 1);
+#pragma unroll
+            for (int i = 0; i < IF; ++i) {
+                const int row = (wi * IF + i) * 16;
+                const bf16x8 fa = TRANS ? tr_operand<ROWA>(A, row, lane)
+                                        : *reinterpret_cast<const bf16x8 *>(A + (row + l16) * 64 + ((g ^ ((l16 >> 2) & 3)) << 4));
+#pragma unroll
+                for (int j = 0; j < JF; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa, acc[i][j], 0, 0, 0);
+            }
         }
     }
+    dma_wait<0>();  // the repeated loads still write this workgroup's LDS
     // a lane holds four neighbouring columns j of row i
     const long out = q.splits > 1 ? split * ((long)q.I * q.J) : 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int ci = i0 + wi * 64 + i * 16 + l16;
+    for (int i = 0; i < IF; ++i) {
+        const int ci = i0 + (wi * IF + i) * 16 + l16;
         if (ci >= q.I) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int cj = j0 + wj * 64 + j * 16 + g * 4;
+        for (int j = 0; j < JF; ++j) {
+            const int cj = j0 + (wj * JF + j) * 16 + g * 4;
             const long at = out + (long)ci * q.J + cj;
             if (q.splits > 1) store_quad((float *)q.c + at, acc[i][j], q.J - cj);
             else store_quad((T *)q.c + at, acc[i][j], q.J - cj);
@@ -252,18 +290,18 @@ __device__ __forceinline__ void bw_product(const BwProduct &q, int bid, uint8_t 
     }
 }
 
-// Both products and the last step of the column sums in one launch: blocks of dX, then of dW, then of db.
-template <int P, class T>
-__global__ __launch_bounds__(256, 2) void e4m3_bw_kernel(BwArgs a) {
-    extern __shared__ uint8_t lds[];  // 64 KB
+// Both products and the last step of the column sums in one launch: blocks of dW (the longer ones), then of dX, then of db.
+template <int P, int IF, int JF, class T>
+__global__ __launch_bounds__(512) void e4m3_bw_kernel(BwArgs a) {
+    extern __shared__ uint8_t lds[];
     int bid = blockIdx.x;
-    if (bid < a.x.blocks) return bw_product<P, false, T>(a.x, bid, lds);
-    bid -= a.x.blocks;
-    if (bid < a.w.blocks) return bw_product<P, true, float>(a.w, bid, lds);
+    if (bid < a.w.blocks) return bw_product<P, true, IF, JF, float>(a.w, bid, lds);
     bid -= a.w.blocks;
-    // db: 32 columns, eight threads of a column add an eighth of the parts each
+    if (bid < a.x.blocks) return bw_product<P, false, IF, JF, T>(a.x, bid, lds);
+    bid -= a.x.blocks;
+    // db: 32 columns, sixteen threads of a column add a sixteenth of the parts each
     float *sums = (float *)lds;
-    const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = bid * 32 + c, per = ceil_div(a.parts, 8);
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = bid * 32 + c, per = ceil_div(a.parts, 16);
     float s = 0.f;
     if (n < a.N)
         for (int t = r * per; t < min((r + 1) * per, a.parts); ++t) s += a.part[(long)t * a.N + n];
@@ -272,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void e4m3_bw_kernel(BwArgs a) {
     if (r || n >= a.N) return;
     s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += sums[k * 32 + c];
+    for (int k = 0; k < 16; ++k) s += sums[k * 32 + c];
     a.db[n] = s;
 }
 
@@ -303,46 +341,60 @@ __global__ __launch_bounds__(256) void e4m3_bw_join_kernel(BwJoin x, BwJoin w) {
     else bw_join<float>(w, blockIdx.x - x.blocks);
 }
 
-// Few output tiles and a long reduction: the reduction is cut into S ranges.  S is the count with the least estimated time: rounds of
-// 512 workgroups (two per compute unit) times a workgroup's steps, plus writing and reading the partial sums.
+static inline int up_to(int v, int a) { return (v + a - 1) / a * a; }
+
+// Tile and splits of both products: those with the least estimated time.  The workgroups of both go to 256 compute units, one each at
+// a time; a reduction is cut into S ranges whose fp32 partial sums are joined in ascending order.
 struct Split {
     int S, per;
 };
-static Split plan_split(int I, int J, int R, int P) {
-    const long tiles = (long)ceil_div(I, 128) * ceil_div(J, 128);
-    const int steps = ceil_div(R, 64);
-    Split best = {1, steps};
+struct BwPlan {
+    int IF, JF;
+    Split sx, sw;
+    size_t planes, part, wx, ww, px, pw, total;
+};
+static double plan_split(int I, int J, int R, int P, int TI, int TJ, Split *out) {
+    const double tiles = (double)ceil_div(I, TI) * ceil_div(J, TJ), part = (TI * TJ) / (256. * 256.) * 0.65 + 0.1;  // us of a part
+    const int steps = ceil_div(R, 32);
     double least = 1e300;
     for (int S = 1; S <= 64 && S <= steps; ++S) {
-        const int per = ceil_div(steps, S), n = ceil_div(steps, per);
-        if (n != S) continue;
-        // us: a step of one piece takes about 0.6 with two workgroups on a compute unit, start and end of a workgroup about 3
-        const double rounds = (double)((tiles * S + 511) / 512), us = rounds * (per * P * 0.6 + 3.0) +
-                                                                     (S > 1 ? 4.0 + 8.0 * S * I * (double)J / 4.0e6 : 0.0);
+        const int per = ceil_div(steps, S);
+        if (ceil_div(steps, per) != S) continue;
+        const double one = per * P * part + 4.0, rounds = tiles * S / 256.;
+        // the last round is rarely full: a share of a workgroup's time on top
+        const double us = (rounds > 1. ? (rounds + 0.4) : 1.) * one + (S > 1 ? 4.0 + 8.0 * S * I * (double)J / 4.0e6 : 0.0);
         if (us < least) {
             least = us;
-            best = {S, per};
+            *out = {S, per};
         }
     }
-    return best;
+    return least;
 }
-
-static inline int up_to(int v, int a) { return (v + a - 1) / a * a; }
-
-struct BwPlan {
-    Split sx, sw;
-    size_t planes, part, px, pw, total;
-};
-static BwPlan plan_bw(int M, int N, int K, int type) {
+static BwPlan plan_bw(int M, int N, int K, int type, bool need_x, bool need_w) {
     const int P = pieces_of(type);
-    BwPlan p;
-    p.sx = plan_split(M, K, N, P);
-    p.sw = plan_split(N, K, M, P);
-    p.planes = align_up((size_t)P * up_to(M, 64) * up_to(N, 128) * 2, 256);
+    BwPlan p = {};
+    double least = 1e300;
+    for (int IF = 4; IF >= 2; IF -= 2)
+        for (int JF = 8; JF >= 4; JF -= JF == 6 ? 2 : 1) {
+            Split sx = {1, 1}, sw = {1, 1};
+            const double us = (need_x ? plan_split(M, K, N, P, IF * 64, JF * 32, &sx) : 0.) +
+                              (need_w ? plan_split(N, K, M, P, IF * 64, JF * 32, &sw) : 0.);
+            if (us < least) {
+                least = us;
+                p.IF = IF;
+                p.JF = JF;
+                p.sx = sx;
+                p.sw = sw;
+            }
+        }
+    const size_t Kp = kp8_of(K);
+    p.planes = align_up((size_t)P * up_to(M, 32) * up_to(N, 32) * 2, 256);
     p.part = align_up((size_t)ceil_div(M, 128) * N * 4, 256);
+    p.wx = need_w ? up_to(M, 32) * Kp * 2 : 0;
+    p.ww = need_x ? up_to(N, 32) * Kp * 2 : 0;
     p.px = p.sx.S > 1 ? align_up((size_t)p.sx.S * M * K * 4, 256) : 0;
     p.pw = p.sw.S > 1 ? align_up((size_t)p.sw.S * N * K * 4, 256) : 0;
-    p.total = p.planes + p.part + p.px + p.pw;
+    p.total = p.planes + p.part + p.wx + p.ww + p.px + p.pw;
     return p;
 }
 
@@ -351,6 +403,21 @@ static void set_split(BwProduct &q, const Split &s, void *out, void *part) {
     q.per_split = s.per;
     q.c = s.S > 1 ? part : out;
     q.blocks = tile_grid(q.num_i, q.num_j) * s.S;
+}
+
+template <int P, int IF, int JF, class T>
+static int launch_products(const BwArgs &g, hipStream_t st) {
+    constexpr int bytes = 4 * (IF * 64 * 64 + 32 * (JF > 4 ? 512 : 256));
+    static PerDeviceOnce once;
+    int dev;
+    if (once.pending(&dev)) {
+        if (hipFuncSetAttribute((const void *)e4m3_bw_kernel<P, IF, JF, T>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+            return fail(PHONLP_ERR_LAUNCH, "linear_e4m3_backward: hipFuncSetAttribute failed");
+        once.mark(dev);
+    }
+    ProfScope ps("e4m3_bw", st);
+    hipLaunchKernelGGL((e4m3_bw_kernel<P, IF, JF, T>), dim3(g.x.blocks + g.w.blocks + g.db_blocks), dim3(512), bytes, st, g);
+    return check_launch("e4m3_bw_kernel");
 }
 
 }  // namespace phonlp
@@ -363,7 +430,13 @@ static bool bw_shape_ok(int M, int N, int K, int type) {
 }
 
 extern "C" size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int type) {
-    return bw_shape_ok(M, N, K, type) ? plan_bw(M, N, K, type).total : 0;
+    if (!bw_shape_ok(M, N, K, type)) return 0;
+    size_t most = 0;  // whichever of dX and dW is asked for
+    for (int need = 1; need < 4; ++need) {
+        const size_t total = plan_bw(M, N, K, type, need & 1, need & 2).total;
+        most = total > most ? total : most;
+    }
+    return most;
 }
 
 extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, const uint32_t *bits, const void *x_codes,
@@ -379,18 +452,31 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
         return fail(PHONLP_ERR_WORKSPACE, "linear_e4m3_backward: workspace too small or not 16-byte aligned");
     if (!dx && !dw && !db) return PHONLP_OK;
     hipStream_t st = as_stream(stream);
-    const BwPlan pl = plan_bw(M, N, K, type);
-    const int Mp = up_to(M, 64), Np = up_to(N, 128), Kp = kp8_of(K), KB4 = kb4_of(K), parts = ceil_div(M, 128);
-    uint8_t *planes = (uint8_t *)ws;
-    float *part = (float *)(planes + pl.planes), *px = (float *)((uint8_t *)part + pl.part), *pw = (float *)((uint8_t *)px + pl.px);
-    // without a mask and with whole tiles, bf16 gradients are their own single piece
-    const bool direct = type == PHONLP_BF16 && !bits && M % 64 == 0 && N % 128 == 0 && lddy % 8 == 0 && lddy < (1 << 24) && !((uintptr_t)dy & 15);
+    const BwPlan pl = plan_bw(M, N, K, type, dx, dw);
+    const int Mp = up_to(M, 32), Np = up_to(N, 32), Kp = kp8_of(K), parts = ceil_div(M, 128);
+    uint8_t *planes = (uint8_t *)ws, *p = planes + pl.planes;
+    float *part = (float *)p;
+    uint8_t *wx = p + pl.part, *ww = wx + pl.wx;
+    float *px = (float *)(ww + pl.ww), *pw = (float *)((uint8_t *)px + pl.px);
+    // without a mask and with whole steps, bf16 gradients are their own single piece
+    const bool direct = type == PHONLP_BF16 && !bits && M % 32 == 0 && N % 32 == 0 && lddy % 8 == 0 && lddy < (1 << 22) && !((uintptr_t)dy & 15);
     const bool make_planes = (dx || dw) && !direct;
+    BwPrep prep = {dy, lddy, bits, make_planes ? (uint16_t *)planes : nullptr, !db ? nullptr : parts == 1 ? db : part,
+                   {(const uint8_t *)x_codes, (const uint8_t *)w_codes}, {x_exponents, w_exponents}, {(__bf16 *)wx, (__bf16 *)ww}, {M, N},
+                   {0, 0}, ceil_div(N, 32), M, N, Mp, Np, Kp, kb4_of(K), ceil_div(Mp, 128), 0};
+    if (make_planes || db) prep.dz_blocks = prep.dz_m * ceil_div(Np, 256);
+    auto wide_blocks = [&](int rows) {
+        const long blocks = ((long)up_to(rows, 32) * (Kp / 16) + 1023) / 1024;
+        return (int)(blocks < 1024 ? blocks : 1024);
+    };
+    if (dw) prep.wide_blocks[0] = wide_blocks(M);
+    if (dx) prep.wide_blocks[1] = wide_blocks(N);
     const uint8_t *a = direct ? (const uint8_t *)dy : planes;
     const long pitch = direct ? lddy * 2 : Np * 2L, plane = (long)Mp * Np * 2;
     BwArgs g = {};
-    g.x = {a, (const uint8_t *)w_codes, w_exponents, nullptr, pitch, plane, M, K, N, Kp, KB4, ceil_div(M, 128), ceil_div(K, 128), 0, 1, 0};
-    g.w = {a, (const uint8_t *)x_codes, x_exponents, nullptr, pitch, plane, N, K, M, Kp, KB4, ceil_div(N, 128), ceil_div(K, 128), 0, 1, 0};
+    const int TI = pl.IF * 64, TJ = pl.JF * 32;
+    g.x = {a, ww, nullptr, pitch, plane, Kp * 2L, M, K, N, ceil_div(M, TI), ceil_div(K, TJ), 0, 1, 0};
+    g.w = {a, wx, nullptr, pitch, plane, Kp * 2L, N, K, M, ceil_div(N, TI), ceil_div(K, TJ), 0, 1, 0};
     if (dx) set_split(g.x, pl.sx, dx, px);
     if (dw) set_split(g.w, pl.sw, dw, pw);
     g.part = part;
@@ -400,20 +486,26 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
     g.db_blocks = db && parts > 1 ? ceil_div(N, 32) : 0;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        constexpr int P = Pieces<T>::N, bytes = 65536;
+        constexpr int P = Pieces<T>::N;
         int rc;
-        if (make_planes || db) {
-            ProfScope ps("e4m3_bw_dz", st);
-            hipLaunchKernelGGL((e4m3_bw_dz_kernel<T>), dim3(ceil_div(Mp, 128), ceil_div(Np, 256)), dim3(256), 0, st, (const T *)dy, lddy,
-                               bits, ceil_div(N, 32), M, N, Mp, Np, make_planes ? (uint16_t *)planes : nullptr,
-                               !db ? nullptr : parts == 1 ? db : part);
-            if ((rc = check_launch("e4m3_bw_dz_kernel"))) return rc;
+        {
+            ProfScope ps("e4m3_bw_prep", st);
+            hipLaunchKernelGGL((e4m3_bw_prep_kernel<T>), dim3(prep.dz_blocks + prep.wide_blocks[0] + prep.wide_blocks[1]), dim3(256), 0, st,
+                               prep);
+            if ((rc = check_launch("e4m3_bw_prep_kernel"))) return rc;
         }
-        const int blocks = g.x.blocks + g.w.blocks + g.db_blocks;
-        if (blocks) {
-            ProfScope ps("e4m3_bw", st);
-            hipLaunchKernelGGL((e4m3_bw_kernel<P, T>), dim3(blocks), dim3(256), bytes, st, g);
-            if ((rc = check_launch("e4m3_bw_kernel"))) return rc;
+        if (g.x.blocks + g.w.blocks + g.db_blocks) {
+            auto by_j = [&](auto f) {
+                constexpr int IF = decltype(f)::value;
+                switch (pl.JF) {
+                    case 4: return launch_products<P, IF, 4, T>(g, st);
+                    case 6: return launch_products<P, IF, 6, T>(g, st);
+                    case 7: return launch_products<P, IF, 7, T>(g, st);
+                    default: return launch_products<P, IF, 8, T>(g, st);
+                }
+            };
+            rc = pl.IF == 2 ? by_j(std::integral_constant<int, 2>{}) : by_j(std::integral_constant<int, 4>{});
+            if (rc) return rc;
         }
         const bool jx = dx && pl.sx.S > 1, jw = dw && pl.sw.S > 1;
         if (!jx && !jw) return PHONLP_OK;

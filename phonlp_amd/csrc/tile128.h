@@ -1,8 +1,5 @@
-// What the kernels on 128-byte rows share (linear_e4m3.hip: 128 codes a row, linear_e4m3_backward.hip: 64 bf16 a row): tiles of
-// [rows][128 bytes] brought to LDS by the LDS-DMA path, and the order in which tiles are handed to workgroups.
-//
-// LDS image of a tile: row r at r * 128, its 16-byte chunk c at slot c ^ (r & 7).  The eight lanes that an LDS read of 16 bytes
-// per lane serves at a time hold eight consecutive rows and the same chunk: eight different slots, no bank conflict.
+// What the matrix kernels of linear_e4m3.hip and linear_e4m3_backward.hip share: loads into LDS past the registers, waits that
+// count them, and the order in which output tiles are handed to workgroups.
 #pragma once
 #include "common.h"
 
@@ -15,20 +12,22 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// 64 lanes x 16 bytes from `base + off` (off per lane) to 1024 consecutive bytes at `lds` (wave-uniform).
-__device__ __forceinline__ void dma16(const uint8_t *base, uint32_t off, uint8_t *lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + off),
-                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+// 64 lanes x 16 bytes from `base + off` (base wave-uniform, off per lane) to 1024 consecutive bytes of LDS (wave-uniform).  Inline
+// asm, as the waits are: the compiler cannot tell the buffers of a ring apart and would let every LDS read wait for every load.
+__device__ __forceinline__ void dma16(const uint8_t *base, uint32_t off, const uint8_t *lds) {
+    const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(base)
+                 : "memory", "m0");
 }
-// All of this wave's loads are done, LDS-DMA among them, and every wave is here.
+// At most N of this wave's loads are still on their way (they arrive in order); then every wave is here, its LDS reads done.
+template <int N>
 __device__ __forceinline__ void dma_wait_barrier() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
     lds_barrier();
 }
-
-// The 16-byte chunk c of row r of a tile image.
-__device__ __forceinline__ i32x4 tile_chunk(const uint8_t *tile, int r, int c) {
-    return *reinterpret_cast<const i32x4 *>(tile + r * 128 + ((c ^ (r & 7)) << 4));
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 #endif
 
