@@ -68,8 +68,8 @@ template <int TM, int TN, int WM, int WN, class T>
 __global__ __launch_bounds__(WM *WN * 64) void linear_e4m3_kernel(E4m3Args a) {
     constexpr int NW = WM * WN, RA = TM / WM / 32, RB = TN / WN / 32, LOADS = (TM + TN) / 8 / NW;
     extern __shared__ uint8_t lds[];  // [2][TM + TN][128]
-    int tm, tn;
-    if (!tile_of(blockIdx.x, a.num_m, a.num_n, 8, &tm, &tn)) return;
+    int tm, tn, split;
+    if (!tile_of(blockIdx.x, a.num_m, a.num_n, 1, 8, &tm, &tn, &split)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const int wm = wave / WN, wn = wave % WN;
     const int m0 = tm * TM, n0 = tn * TN;
@@ -178,7 +178,7 @@ static int launch_tile(E4m3Args a, hipStream_t st) {
     }
     a.num_m = ceil_div(a.M, TM);
     a.num_n = ceil_div(a.N, TN);
-    hipLaunchKernelGGL((linear_e4m3_kernel<TM, TN, WM, WN, T>), dim3(tile_grid(a.num_m, a.num_n)), dim3(WM * WN * 64), bytes, st, a);
+    hipLaunchKernelGGL((linear_e4m3_kernel<TM, TN, WM, WN, T>), dim3(tile_grid(a.num_m, a.num_n, 1)), dim3(WM * WN * 64), bytes, st, a);
     return check_launch("linear_e4m3_kernel");
 }
 

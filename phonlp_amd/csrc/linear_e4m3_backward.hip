@@ -203,16 +203,16 @@ __device__ __forceinline__ uint32_t tr_offset(int u, int lane, long pitch, long 
     return (uint32_t)r * (uint32_t)pitch + (uint32_t)min((long)c * 16, last);
 }
 
-// Tile of 64 IF x 32 JF, eight waves (4 x 2) of 16 IF x 16 JF, steps of 32 r.  Both operands come by LDS-DMA, three parts (a step and
-// piece) ahead in rings of four; the waits count loads, so that two parts stay in flight.
+// Tile of 64 IF x 32 JF, eight waves (4 x 2) of 16 IF x 16 JF, steps of 32 r.  Both operands come by LDS-DMA into rings of four parts (a
+// step and piece), and from there into one of two register sets while the other is multiplied; the waits count loads, so that two
+// parts stay in flight across each barrier.
 template <int P, bool TRANS, int IF, int JF, class T>
 __device__ __forceinline__ void bw_product(const BwProduct &q, int bid, uint8_t *lds) {
     constexpr int TI = IF * 64, TJ = JF * 32, ROWA = TRANS ? TI * 2 : 64, ROWB = JF > 4 ? 512 : 256, SA = TI * 64, SB = 32 * ROWB;
     constexpr int NA = SA / 8192, NB = SB / 8192;  // loads per wave
     uint8_t *ta = lds, *tb = lds + 4 * SA;
-    int ti, tj;
-    const int tiles8 = (q.num_i * q.num_j + 7) / 8 * 8, split = bid / tiles8;
-    if (!tile_of(bid - split * tiles8, q.num_i, q.num_j, 8, &ti, &tj)) return;
+    int ti, tj, split;
+    if (!tile_of(bid, q.num_i, q.num_j, q.splits, 8, &ti, &tj, &split)) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wi = wave >> 1, wj = wave & 1, i0 = ti * TI, j0 = tj * TJ;
     const int first = split * q.per_split, last = min(first + q.per_split, ceil_div(q.R, 32)), steps = last - first, parts = steps * P;
@@ -227,49 +227,92 @@ __device__ __forceinline__ void bw_product(const BwProduct &q, int bid, uint8_t 
 #pragma unroll
     for (int k = 0; k < NB; ++k) ob[k] = tr_offset<ROWB>(wave + k * 8, lane, q.pitch_b, q.pitch_b - 16 - j0 * 2L);
     const uint8_t *ab = q.a + (TRANS ? i0 * 2L : i0 * q.pitch_a), *bb = q.b + j0 * 2L;
-    // behind the end the last part is loaded again: the number of loads in flight stays what the waits count
-    auto load = [&](int t, bool b) {
+    // Load `k` of part t: its A's NA, then, where a step begins, B's NB.  Behind the end the last part is loaded again: the number of
+    // loads in flight stays what the waits count.
+    auto load = [&](int t, int k) {
         const int slot = t & 3, slot_b = t / P & 3;
         t = min(t, parts - 1);
         const int s = t / P, p = t - s * P;
-        if (b) {
-#pragma unroll
-            for (int k = 0; k < NB; ++k) dma16(bb + (first + s) * (32 * q.pitch_b), ob[k], tb + slot_b * SB + (wave + k * 8) * 1024);
-        }
-#pragma unroll
-        for (int k = 0; k < NA; ++k)
-            dma16(ab + p * q.plane + (first + s) * (TRANS ? 32 * q.pitch_a : 64L), oa[k], ta + slot * SA + (wave + k * 8) * 1024);
+        if (k < NA)
+            dma16(ab + p * q.plane + (first + s) * (TRANS ? 32 * q.pitch_a : 64L), oa[k < NA ? k : 0], ta + slot * SA + (wave + k * 8) * 1024);
+        else
+            dma16(bb + (first + s) * (32 * q.pitch_b), ob[k < NA ? 0 : k - NA], tb + slot_b * SB + (wave + (k - NA) * 8) * 1024);
     };
     f32x4 acc[IF][JF];
 #pragma unroll
     for (int i = 0; i < IF; ++i)
 #pragma unroll
         for (int j = 0; j < JF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct A {
+        bf16x8 f[IF];
+    };
+    struct B {
+        bf16x8 f[JF];
+    };
+    auto read_a = [&](int t, int i, A &x) {
+        const uint8_t *tile = ta + (t & 3) * SA;
+        const int row = (wi * IF + i) * 16;
+        x.f[i] = TRANS ? tr_operand<ROWA>(tile, row, lane)
+                       : *reinterpret_cast<const bf16x8 *>(tile + (row + l16) * 64 + ((g ^ ((l16 >> 2) & 3)) << 4));
+    };
+    auto read_b = [&](int s, int j, B &x) { x.f[j] = tr_operand<ROWB>(tb + (s & 3) * SB, (wj * JF + j) * 16, lane); };
+    // Part t: its operands are in registers; those of part t + 1 are read while it is multiplied, and its own buffer is filled again.
+    // Loads (60 to 180 cycles each to issue) and LDS reads stand between the matrix instructions, the reads well before the barrier.
+    auto part = [&](int t, auto pc, const A &a, A &next_a, const B &b, B &next_b) {
+        constexpr int p = decltype(pc)::value;
+        constexpr int LOADS = NA + ((p + 4) % P == 0 ? NB : 0), READS = IF + (p + 1 == P ? JF : 0), EARLY = IF - (IF > 2 ? 1 : 0);
+        // in flight behind part t + 1: parts t + 2 and t + 3, with B where a step begins
+        dma_wait_barrier<2 * NA + (P == 1 ? 2 : P == 3 && p == 2 ? 0 : 1) * NB>();
 #pragma unroll
-    for (int t = 0; t < 3; ++t) load(t, t % P == 0);
-    for (int s = 0; s < steps; ++s) {
-        bf16x8 fb[JF];
+        for (int i = 0; i < IF; ++i) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            // in flight behind part t: parts t + 1 and t + 2, with B where a step begins
-            constexpr int two = 2 * NA;
-            if (P == 1) dma_wait_barrier<two + 2 * NB>();
-            else if (P == 2 || p > 0) dma_wait_barrier<two + NB>();
-            else dma_wait_barrier<two>();
-            const int t = s * P + p;
-            load(t + 3, (p + 3) % P == 0);
-            const uint8_t *A = ta + (t & 3) * SA, *B = tb + (s & 3) * SB;
-            if (p == 0) {
+            for (int k = LOADS * i / IF; k < LOADS * (i + 1) / IF; ++k) load(t + 4, k);
 #pragma unroll
-                for (int j = 0; j < JF; ++j) fb[j] = tr_operand<ROWB>(B, (wj * JF + j) * 16, lane);
+            for (int k = READS * i / EARLY; k < READS * (i + 1) / EARLY; ++k) {
+                if (k >= READS) break;
+                if (k < IF) read_a(t + 1, k, next_a);
+                else read_b((t + 1) / P, k - IF, next_b);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < IF; ++i) {
-                const int row = (wi * IF + i) * 16;
-                const bf16x8 fa = TRANS ? tr_operand<ROWA>(A, row, lane)
-                                        : *reinterpret_cast<const bf16x8 *>(A + (row + l16) * 64 + ((g ^ ((l16 >> 2) & 3)) << 4));
+            for (int j = 0; j < JF; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.f[j], a.f[i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
 #pragma unroll
-                for (int j = 0; j < JF; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa, acc[i][j], 0, 0, 0);
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int k = 0; k < NA + (t % P == 0 ? NB : 0); ++k) load(t, k);
+    A a0, a1;
+    B b0, b1;
+    dma_wait_barrier<3 * NA + (P == 1 ? 3 : 1) * NB>();
+#pragma unroll
+    for (int j = 0; j < JF; ++j) read_b(0, j, b0);
+#pragma unroll
+    for (int i = 0; i < IF; ++i) read_a(0, i, a0);
+    using p0 = std::integral_constant<int, 0>;
+    using p1 = std::integral_constant<int, P == 1 ? 0 : 1>;
+    using p2 = std::integral_constant<int, 2>;
+    // two steps a turn, so that the two register sets stand where they are
+    for (int t = 0; t < parts;) {
+        if constexpr (P == 1) {
+            part(t++, p0{}, a0, a1, b0, b1);
+            if (t < parts) part(t++, p0{}, a1, a0, b1, b0);
+        } else if constexpr (P == 2) {
+            part(t++, p0{}, a0, a1, b0, b1);
+            part(t++, p1{}, a1, a0, b0, b1);
+            if (t < parts) {
+                part(t++, p0{}, a0, a1, b1, b0);
+                part(t++, p1{}, a1, a0, b1, b0);
+            }
+        } else {
+            part(t++, p0{}, a0, a1, b0, b1);
+            part(t++, p1{}, a1, a0, b0, b1);
+            part(t++, p2{}, a0, a1, b0, b1);
+            if (t < parts) {
+                part(t++, p0{}, a1, a0, b1, b0);
+                part(t++, p1{}, a0, a1, b1, b0);
+                part(t++, p2{}, a1, a0, b1, b0);
             }
         }
     }
@@ -402,7 +445,7 @@ static void set_split(BwProduct &q, const Split &s, void *out, void *part) {
     q.splits = s.S;
     q.per_split = s.per;
     q.c = s.S > 1 ? part : out;
-    q.blocks = tile_grid(q.num_i, q.num_j) * s.S;
+    q.blocks = tile_grid(q.num_i, q.num_j, s.S);
 }
 
 template <int P, int IF, int JF, class T>

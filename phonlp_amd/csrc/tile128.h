@@ -31,19 +31,22 @@ __device__ __forceinline__ void dma_wait() {
 }
 #endif
 
-// The tile of workgroup `bid` out of num_m x num_n.  Workgroups go to the eight XCDs in turn and each XCD has its own L2: every XCD
-// gets a contiguous share of the tile order, and the order runs through groups of `gm` row tiles, column by column, so that the
-// workgroups that run together on one XCD share operand rows.  Returns false for the surplus workgroups of the rounded-up grid.
-__device__ __forceinline__ bool tile_of(int bid, int num_m, int num_n, int gm, int *tm, int *tn) {
-    const int total = num_m * num_n, share = (total + 7) / 8;
-    const int id = (bid & 7) * share + (bid >> 3);
+// The tile and the range of the reduction of workgroup `bid`, out of num_m x num_n tiles and `splits` ranges.  Workgroups go to the
+// eight XCDs in turn and each XCD has its own L2: every XCD gets a contiguous share of the order, which runs range by range, in a
+// range through groups of `gm` row tiles, in a group column by column, so that the workgroups that run together on one XCD share
+// operand rows.  Returns false for the surplus workgroups of the rounded-up grid.
+__device__ __forceinline__ bool tile_of(int bid, int num_m, int num_n, int splits, int gm, int *tm, int *tn, int *split) {
+    const int tiles = num_m * num_n, total = tiles * splits, share = (total + 7) / 8;
+    int id = (bid & 7) * share + (bid >> 3);
     if ((bid >> 3) >= share || id >= total) return false;
+    *split = id / tiles;
+    id -= *split * tiles;
     const int per_group = gm * num_n, g = id / per_group, in = id - g * per_group;
     const int rows = min(gm, num_m - g * gm);
     *tm = g * gm + in % rows;
     *tn = in / rows;
     return true;
 }
-inline int tile_grid(int num_m, int num_n) { return (num_m * num_n + 7) / 8 * 8; }
+inline int tile_grid(int num_m, int num_n, int splits) { return (num_m * num_n * splits + 7) / 8 * 8; }
 
 }  // namespace phonlp
