@@ -12,11 +12,23 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// Byte offset of a pointer into LDS: the low half of its flat address.
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t *p) { return (uint32_t)(uintptr_t)p; }
+
 // 64 lanes x 16 bytes from `base + off` (base wave-uniform, off per lane) to 1024 consecutive bytes of LDS (wave-uniform).  Inline
 // asm, as the waits are: the compiler cannot tell the buffers of a ring apart and would let every LDS read wait for every load.
 __device__ __forceinline__ void dma16(const uint8_t *base, uint32_t off, const uint8_t *lds) {
-    const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds;
+    const uint32_t at = lds_offset(lds);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+// The same with four bytes per lane, of the lanes in `mask` alone.  For waves whose lanes are all active: exec is -1 afterwards (a
+// branch around the load would end the basic block, and the compiler moves matrix instructions across block ends).
+__device__ __forceinline__ void dma4(const uint8_t *base, uint32_t off, const uint8_t *lds, unsigned long long mask) {
+    const uint32_t at = lds_offset(lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1" ::"s"(
+                     __builtin_amdgcn_readfirstlane(at)),
+                 "v"(off), "s"(base), "s"(mask)
                  : "memory", "m0");
 }
 // At most N of this wave's loads are still on their way (they arrive in order); then every wave is here, its LDS reads done.
