@@ -35,7 +35,7 @@ __device__ __forceinline__ float scale_of(int exponents) { return __int_as_float
 
 // Bias, ReLU and the rounding to T of four neighbouring values.
 template <class T>
-__device__ __forceinline__ typename Vec<T, 4>::type finish(f32x4 v, const float (&bias)[4], int relu) {
+__device__ __forceinline__ typename Vec<T, 4>::type finish(f32x4 v, const f32x4 &bias, int relu) {
     typename Vec<T, 4>::type t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -46,72 +46,90 @@ __device__ __forceinline__ typename Vec<T, 4>::type finish(f32x4 v, const float 
     return t;
 }
 
-// Up to 16 bytes of a row of Y, and their bits (column n in bit n % 8 of byte n / 8 of a row: the words of phonlp_linear_e4m3).
-template <class T>
-__device__ __forceinline__ void store_row(const E4m3Args &a, int m, int n, const typename Vec<T, 16 / sizeof(T)>::type &v) {
-    constexpr int VEC = 16 / sizeof(T);
-    if (m >= a.M) return;
-    T *y = (T *)a.y + (long)m * a.N + n;
-    const int left = a.N - n;
-    if (left >= VEC) {
-        *reinterpret_cast<typename Vec<T, VEC>::type *>(y) = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (i < left) y[i] = v[i];
-    }
-    if (!a.bits) return;
-    int b = 0;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) b |= i < left && (float)v[i] > 0.f ? 1 << i : 0;
-    if (VEC == 4) {  // a byte is two lanes' four columns
-        b |= __shfl_down(b, 1) << 4;
-        if (n & 4) return;
-    }
-    if (n >> 3 < a.row_bytes) a.bits[(long)m * a.row_bytes + (n >> 3)] = (uint8_t)b;
-}
-
 // Tile of TM x TN, eight waves (4 x 2) of TM / 4 x TN / 2.  A block of 128 codes of every row comes by LDS-DMA in whole 128-byte lines
 // into one of two buffers, and goes through registers in two parts of 64.  The codes of a part are read from LDS while the part
 // before is multiplied, so one barrier a block, before its second part, does: there block kb + 1 has landed, and as every wave
 // has all of block kb in registers, its buffer takes block kb + 2, a whole block's time ahead.
-// Four blocks' exponents of a row are one dword; those of the tile's rows lie in a ring of four LDS slots, and each block brings a
-// quarter of the next slot's.
+// A workgroup takes tile after tile (PERSIST): behind a tile's last block come the next tile's first two, so that they land while the
+// results are written, and the first wait behind the results lets their stores go on.
+// Four blocks' exponents of a row are one dword, brought with every fourth block into a ring of four LDS slots; the bias comes into
+// LDS with a tile's first block.
 //
 // LDS image of a block: row r at r * 128, its 16-byte chunk c at slot c ^ ((r >> 1) & 7): sixteen rows' chunks c lie in all 64 banks.
 template <int TM, int TN, class T>
+struct E4m3Tile {
+    static constexpr bool PIPE8 = sizeof(T) == 2;  // which matrix pipe (above)
+    static constexpr int ROWS = TM + TN, SIZE = ROWS * 128, SLOTS = 4 * ROWS * 4, PATCH = 2048;
+    // not the smaller tile, which shares a compute unit with a second workgroup, nor the bf16 pipe, whose registers are all in use
+    static constexpr bool PERSIST = TM == 256 && PIPE8;
+    static constexpr int BIAS = 2 * TN * 4, BYTES = 2 * SIZE + SLOTS + BIAS + (PERSIST ? 8 * PATCH : 0);
+    static constexpr int STORES = (TM / 4) * (TN / 2) * (int)sizeof(T) / 1024;  // of a wave, for a whole tile without bits
+};
+
+template <int TM, int TN, class T>
 __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
-    constexpr bool PIPE8 = sizeof(T) == 2;  // which matrix pipe (above)
-    constexpr int ROWS = TM + TN, SIDE = PIPE8 ? 32 : 16, FA = TM / 4 / SIDE, FB = TN / 2 / SIDE, LOADS = ROWS / 64, SIZE = ROWS * 128;
-    extern __shared__ uint8_t lds[];  // [2][ROWS][128] codes, [4][ROWS] exponents; then the waves' output patches
-    uint8_t *slots = lds + 2 * SIZE;
-    int tm, tn, split;
-    if (!tile_of(blockIdx.x, a.num_m, a.num_n, 1, 8, &tm, &tn, &split)) return;
+    using Tile = E4m3Tile<TM, TN, T>;
+    constexpr bool PIPE8 = Tile::PIPE8, PERSIST = Tile::PERSIST;
+    constexpr int ROWS = Tile::ROWS, SIZE = Tile::SIZE, SIDE = PIPE8 ? 32 : 16, FA = TM / 4 / SIDE, FB = TN / 2 / SIDE, LOADS = ROWS / 64;
+    extern __shared__ uint8_t lds[];  // [2][ROWS][128] codes, [4][ROWS] exponents, [2][TN] bias, the waves' output patches (or in the codes' place)
+    uint8_t *slots = lds + 2 * SIZE, *biases = slots + Tile::SLOTS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int wm = wave >> 1, wn = wave & 1, ls = lane & (SIDE - 1), lg = lane / SIDE, m0 = tm * TM, n0 = tn * TN;
+    const int wm = wave >> 1, wn = wave & 1, ls = lane & (SIDE - 1), lg = lane / SIDE;
     const int blocks = a.Kp / 128, groups = a.KB4 / 4;
 
-    // rows behind the matrix read its last row: their products are not stored
-    const uint8_t *xb = a.x + (long)m0 * a.Kp, *wb = a.w + (long)n0 * a.Kp;
-    uint32_t off[LOADS];
-#pragma unroll
-    for (int k = 0; k < LOADS; ++k) {
-        const int r = (wave + k * 8) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-        off[k] = (uint32_t)(r < TM ? min(r, a.M - 1 - m0) : min(r - TM, a.N - 1 - n0)) * (uint32_t)a.Kp + c * 16;
-    }
-    auto load = [&](int kb, int k) {  // behind the end the last block again
-        const int r8 = wave + k * 8;
-        dma16((r8 * 8 < TM ? xb : wb) + min(kb, blocks - 1) * 128, off[k], lds + (kb & 1) * SIZE + r8 * 1024);
+    struct Place {  // a tile's first row and column
+        int m, n;
     };
-    // Exponents of the group G of four blocks: of the eighth of the tile's rows that this wave brings, quarter z (of `of`).
-    auto load_exponents = [&](int G, int z, int of) {
-        const int to = (G & 3) * ROWS, g = min(G, groups - 1) * 4;
+    auto place = [&](int bid, Place &t) {
+        int tm, tn, split;
+        if (!tile_of(bid, a.num_m, a.num_n, 1, 8, &tm, &tn, &split)) return false;
+        t.m = tm * TM;
+        t.n = tn * TN;
+        return true;
+    };
+    int bid = blockIdx.x;
+    Place now, next;
+    if (!place(bid, now)) return;
+
+    // Where a tile's block kb is loaded from; rows behind the matrix read its last one: their products are not stored.
+    struct From {
+        const uint8_t *x, *w, *xe, *we;
+        uint32_t last_x, last_w;  // byte offsets of the last rows
+        int last_m, last_n;
+    };
+    auto from = [&](const Place &t, int kb) {
+        From f;
+        f.x = a.x + (long)t.m * a.Kp + kb * 128;
+        f.w = a.w + (long)t.n * a.Kp + kb * 128;
+        f.xe = a.xe + (long)t.m * a.KB4 + (kb >> 2) * 4;
+        f.we = a.we + (long)t.n * a.KB4 + (kb >> 2) * 4;
+        f.last_m = min(TM, a.M - t.m) - 1;
+        f.last_n = min(TN, a.N - t.n) - 1;
+        f.last_x = (uint32_t)f.last_m * (uint32_t)a.Kp;
+        f.last_w = (uint32_t)f.last_n * (uint32_t)a.Kp;
+        return f;
+    };
+    // load k of a block: rows 8 (wave + 8 k) + lane / 8
+    const uint32_t row0 = (uint32_t)(wave * 8 + (lane >> 3)) * (uint32_t)a.Kp, chunk = ((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7)) << 4;
+    auto load = [&](const From &f, int buf, int k) {
+        const bool w = k >= TM / 64;
+        const uint32_t row = row0 + (uint32_t)(w ? k - TM / 64 : k) * 64u * (uint32_t)a.Kp;
+        dma16(w ? f.w : f.x, min(row, w ? f.last_w : f.last_x) + chunk, lds + buf * SIZE + (wave + k * 8) * 1024);
+    };
+    // the exponents of its group, of the eighth of the tile's rows that this wave brings
+    auto load_exponents = [&](const From &f, int slot, bool on) {
+        static_assert(TM == TN, "both operands' rows alike");
+        constexpr int each = TM / 8;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const int rows = (w ? TN : TM) / 8 / of, r = (w ? TN : TM) / 8 * wave + z * rows, last = w ? a.N - 1 - n0 : a.M - 1 - m0;
-            dma4((w ? a.we + (long)n0 * a.KB4 : a.xe + (long)m0 * a.KB4) + g, (uint32_t)min(r + lane, last) * (uint32_t)a.KB4,
-                 slots + (to + (w ? TM : 0) + r) * 4, (1ull << rows) - 1);
-        }
+        for (int w = 0; w < 2; ++w)
+            dma4(w ? f.we : f.xe, (uint32_t)min(wave * each + lane, w ? f.last_n : f.last_m) * (uint32_t)a.KB4,
+                 slots + ((slot & 3) * ROWS + w * TM + wave * each) * 4, on ? (1ull << each) - 1 : 0ull);
+    };
+
+    auto load_bias = [&](const Place &t, int which, bool on) {
+        constexpr int each = TN / 8;
+        dma4((const uint8_t *)(a.bias + t.n), (uint32_t)min(wave * each + lane, min(TN, a.N - t.n) - 1) * 4u,
+             biases + (which * TN + wave * each) * 4, on && a.bias ? (1ull << each) - 1 : 0ull);
     };
 
     // lane (ls, lg) holds row ls of a fragment: of a part's 64 codes 32 from 32 lg (8-bit pipe), or 16 from 16 lg, eight for each of two
@@ -133,16 +151,16 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
     struct Scales {
         int a[FA], b[FB];
     };
-    auto read_a = [&](int kb, int p, int i, A &x) {
+    auto read_a = [&](int buf, int p, int i, A &x) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) x.f[i][h] = *reinterpret_cast<const i32x4 *>(lds + (kb & 1) * SIZE + at_a[p][h] + i * SIDE * 128);
+        for (int h = 0; h < H; ++h) x.f[i][h] = *reinterpret_cast<const i32x4 *>(lds + buf * SIZE + at_a[p][h] + i * SIDE * 128);
     };
-    auto read_b = [&](int kb, int p, int j) {
+    auto read_b = [&](int buf, int p, int j) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) b[j][h] = *reinterpret_cast<const i32x4 *>(lds + (kb & 1) * SIZE + at_b[p][h] + j * SIDE * 128);
+        for (int h = 0; h < H; ++h) b[j][h] = *reinterpret_cast<const i32x4 *>(lds + buf * SIZE + at_b[p][h] + j * SIDE * 128);
     };
-    auto read_scales = [&](int kb, Scales &s) {  // of block kb, in the lowest byte
-        const int *e = reinterpret_cast<const int *>(slots) + ((kb >> 2) & 3) * ROWS + ls, shift = (kb & 3) * 8;
+    auto read_scales = [&](int kb, int slot, Scales &s) {  // of block kb, in the lowest byte
+        const int *e = reinterpret_cast<const int *>(slots) + (slot & 3) * ROWS + ls, shift = (kb & 3) * 8;
 #pragma unroll
         for (int i = 0; i < FA; ++i) s.a[i] = (unsigned)e[wm * (TM / 4) + i * SIDE] >> shift;
 #pragma unroll
@@ -151,24 +169,25 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
 
     typedef std::conditional_t<PIPE8, f32x16, f32x4> Acc;
     Acc acc[FA][FB];
-#pragma unroll
-    for (int i = 0; i < FA; ++i)
-#pragma unroll
-        for (int j = 0; j < FB; ++j)
-#pragma unroll
-            for (int r = 0; r < SIDE * SIDE / 64; ++r) acc[i][j][r] = 0.f;
+    int buf = 0, slot = 0, which = 0;  // of the block at hand; of this tile's first group; of its bias
 
-    // Part p of block kb: its codes are in `now` and b; loads, and LDS reads of the next part's codes into registers that are done
+    // Part p of block kb: its codes are in `now_a` and b; loads, and LDS reads of the next part's codes into registers that are done
     // with, stand between its matrix instructions.
-    auto part = [&](int kb, auto pc, A &now, A &next, const Scales &s) {
+    auto part = [&](int kb, auto pc, A &now_a, A &next_a, const Scales &s) {
         constexpr int p = decltype(pc)::value;
-        const int nk = kb + p;  // the next part: 1 - p of block nk
-        if (p == 1) dma_wait_barrier<0>();
+        const int nbuf = buf ^ p;  // the next part: 1 - p of this block or the next
+        const bool here = kb + 2 < blocks;  // block kb + 2, or the next tile's
+        const int v = here ? kb + 2 : min(kb + 2 - blocks, blocks - 1);
+        From f;
+        if (p == 1) f = from(Place{here ? now.m : next.m, here ? now.n : next.n}, v);
         auto loads = [&](int z, int of) {  // the share of step z of `of`
             if (p == 0) return;
 #pragma unroll
-            for (int k = LOADS * z / of; k < LOADS * (z + 1) / of; ++k) load(kb + 2, k);
-            if (z == of - 1) load_exponents(((kb + 1) >> 2) + 1, (kb + 1) & 3, 4);
+            for (int k = LOADS * z / of; k < LOADS * (z + 1) / of; ++k) load(f, buf, k);
+            if (z == of - 1) {
+                load_exponents(f, slot + (here ? 0 : groups) + (v >> 2), (v & 3) == 0);
+                if (PERSIST) load_bias(next, which ^ 1, !here && v == 0);
+            }
         };
         if constexpr (PIPE8) {
 #pragma unroll
@@ -176,16 +195,16 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
                 loads(j, FB);
                 if (j == 0) {
 #pragma unroll
-                    for (int i = 0; i < FA; ++i) read_a(nk, 1 - p, i, next);
+                    for (int i = 0; i < FA; ++i) read_a(nbuf, 1 - p, i, next_a);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < FA; ++i)
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
                         __builtin_shufflevector(b[j][0], b[j][1], 0, 1, 2, 3, 4, 5, 6, 7),
-                        __builtin_shufflevector(now.f[i][0], now.f[i][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][j], 0, 0, 0, s.b[j], 0, s.a[i]);
+                        __builtin_shufflevector(now_a.f[i][0], now_a.f[i][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][j], 0, 0, 0, s.b[j], 0, s.a[i]);
                 __builtin_amdgcn_sched_barrier(0);
-                read_b(nk, 1 - p, j);
+                read_b(nbuf, 1 - p, j);
             }
         } else {
             constexpr int HB = FB / 2, STEPS = 4 * FA;  // half of B's fragments at a time: registers
@@ -193,7 +212,7 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
             for (int q = 0; q < 2; ++q) {
                 bf16x8 fa[FA];
 #pragma unroll
-                for (int i = 0; i < FA; ++i) fa[i] = widen(now.f[i][0][2 * q], now.f[i][0][2 * q + 1], scale_of(s.a[i]));
+                for (int i = 0; i < FA; ++i) fa[i] = widen(now_a.f[i][0][2 * q], now_a.f[i][0][2 * q + 1], scale_of(s.a[i]));
 #pragma unroll
                 for (int jh = 0; jh < 2; ++jh) {
                     bf16x8 fb[HB];
@@ -204,10 +223,10 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
                     }
                     if (q == 1) {  // these codes of this part are used up
 #pragma unroll
-                        for (int k = 0; k < HB; ++k) read_b(nk, 1 - p, jh * HB + k);
+                        for (int k = 0; k < HB; ++k) read_b(nbuf, 1 - p, jh * HB + k);
                         if (jh == 0) {
 #pragma unroll
-                            for (int k = 0; k < FA; ++k) read_a(nk, 1 - p, k, next);
+                            for (int k = 0; k < FA; ++k) read_a(nbuf, 1 - p, k, next_a);
                         }
                     }
 #pragma unroll
@@ -223,55 +242,115 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
             }
         }
     };
+    using first_part = std::integral_constant<int, 0>;
+    using second_part = std::integral_constant<int, 1>;
 
-    load_exponents(0, 0, 1);
+    {
+        const From f = from(now, 0);
 #pragma unroll
-    for (int k = 0; k < LOADS; ++k) load(0, k);
+        for (int k = 0; k < LOADS; ++k) load(f, 0, k);
+        load_exponents(f, 0, true);
+        load_bias(now, 0, true);
+    }
     dma_wait_barrier<0>();
+    bool more = PERSIST && place(bid + gridDim.x, next), whole = false;
+    if (!more) next = now;
+    {
+        const From f = from(blocks > 1 ? now : next, blocks > 1 ? 1 : 0);
 #pragma unroll
-    for (int k = 0; k < LOADS; ++k) load(1, k);
-    load_exponents(1, 0, 4);
+        for (int k = 0; k < LOADS; ++k) load(f, 1, k);
+        load_exponents(f, groups, blocks == 1);
+    }
     A a0, a1;
     Scales s;
 #pragma unroll
     for (int i = 0; i < FA; ++i) read_a(0, 0, i, a0);
 #pragma unroll
     for (int j = 0; j < FB; ++j) read_b(0, 0, j);
-    read_scales(0, s);
-    for (int kb = 0; kb < blocks; ++kb) {
-        part(kb, std::integral_constant<int, 0>{}, a0, PIPE8 ? a1 : a0, s);
-        part(kb, std::integral_constant<int, 1>{}, PIPE8 ? a1 : a0, a0, s);
-        read_scales(kb + 1, s);  // a next group's came with blocks up to kb + 1, which have landed
-    }
-    dma_wait_barrier<0>();  // the repeated loads have landed and every wave is done with the buffers
+    read_scales(0, 0, s);
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+            for (int j = 0; j < FB; ++j)
+#pragma unroll
+                for (int r = 0; r < SIDE * SIDE / 64; ++r) acc[i][j][r] = 0.f;
+        auto block = [&](int kb, auto pc) {
+            constexpr bool first = decltype(pc)::value;
+            part(kb, first_part{}, a0, PIPE8 ? a1 : a0, s);
+            // behind a whole tile's results the loads of block 1 are older than exactly its stores
+            if (first && whole) dma_wait_barrier<Tile::STORES>();
+            else dma_wait_barrier<0>();
+            part(kb, second_part{}, PIPE8 ? a1 : a0, a0, s);
+            buf ^= 1;
+            const int v = kb + 1 < blocks ? kb + 1 : 0;
+            read_scales(v, slot + (kb + 1 < blocks ? 0 : groups) + (v >> 2), s);  // landed with block kb + 1
+        };
+        if (PERSIST) block(0, std::true_type{});
+        for (int kb = PERSIST; kb < blocks; ++kb) block(kb, std::false_type{});
+        slot += groups;
 
-    // Through LDS, a patch of SIDE rows per wave, so that Y is written in whole row segments of 16 bytes per lane.
-    constexpr int VEC = 16 / sizeof(T), COLS = TN / 2, PITCH = COLS * sizeof(T) + 16, LANES = COLS / VEC;
-    static_assert(8 * SIDE * PITCH <= 4 * ROWS * 64 + 4 * ROWS * 4, "the patches must fit");
-    uint8_t *patch = lds + wave * (SIDE * PITCH);
+        // Through LDS, a patch of a wave's own, so that Y is written in row segments of 64 (16-bit) or 128 bytes.
+        if (!PERSIST) dma_wait_barrier<0>();  // the patches take the codes' place
+        whole = now.m + TM <= a.M && now.n + TN <= a.N;
+        uint8_t *patch = (PERSIST ? biases + Tile::BIAS : lds) + wave * Tile::PATCH;
+        constexpr int VEC = 16 / sizeof(T), LANES = 32 / VEC, ROWB = 32 * sizeof(T), JJ = 32 / SIDE;
+        auto swizzle = [](int r, int c) { return r * ROWB + ((sizeof(T) == 2 ? c ^ ((r >> 2) & 3) : c ^ ((r >> 1) & 7)) << 4); };
 #pragma unroll
-    for (int i = 0; i < FA; ++i) {
+        for (int jq = 0; jq < FB / JJ; ++jq) {
+            const int nw = now.n + wn * (TN / 2) + jq * 32;
+            constexpr int QUADS = SIDE * SIDE * JJ / 256;
+            f32x4 bias[QUADS];  // of four neighbouring columns
 #pragma unroll
-        for (int j = 0; j < FB; ++j) {
+            for (int q = 0; q < QUADS; ++q) {
+                bias[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+                const int c = wn * (TN / 2) + jq * 32 + (PIPE8 ? 8 * q : 16 * q) + 4 * lg;
+                if (a.bias) bias[q] = *reinterpret_cast<const f32x4 *>(biases + (which * TN + c) * 4);
+            }
 #pragma unroll
-            for (int q = 0; q < SIDE * SIDE / 256; ++q) {  // four neighbouring columns of row ls
-                const int c = j * SIDE + (PIPE8 ? 8 * q + 4 * lg : 4 * lg), n = n0 + wn * COLS + c;
-                float bias[4];
+            for (int i = 0; i < FA; ++i) {
+                const int mw = now.m + wm * (TM / 4) + i * SIDE;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) bias[k] = a.bias && n + k < a.N ? a.bias[n + k] : 0.f;
-                const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                *reinterpret_cast<typename Vec<T, 4>::type *>(patch + ls * PITCH + c * sizeof(T)) = finish<T>(v, bias, a.relu);
+                for (int q = 0; q < QUADS; ++q) {  // four neighbouring columns of row ls
+                    const int c = (PIPE8 ? 8 * q : 16 * q) + 4 * lg, j = jq * JJ + (PIPE8 ? 0 : q), r = PIPE8 ? 4 * q : 0;
+                    const f32x4 v = {acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+                    *reinterpret_cast<typename Vec<T, 4>::type *>(patch + swizzle(ls, c / VEC) + (c % VEC) * sizeof(T)) =
+                        finish<T>(v, bias[q], a.relu);
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int r0 = 0; r0 < SIDE; r0 += 64 / LANES) {
+                    const int r = r0 + lane / LANES, c = lane % LANES, m = mw + r, n = nw + c * VEC;
+                    if (m >= a.M) continue;
+                    const T *from = reinterpret_cast<const T *>(patch + swizzle(r, c));
+                    T *to = (T *)a.y + (long)m * a.N + n;
+                    const auto v = *reinterpret_cast<const typename Vec<T, VEC>::type *>(from);
+                    const int left = a.N - n;
+                    if (left >= VEC) *reinterpret_cast<typename Vec<T, VEC>::type *>(to) = v;
+                    else
+#pragma unroll 1
+                        for (int k = 0; k < left; ++k) to[k] = from[k];
+                    if (a.bits) {
+                        int bits = 0;
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) bits |= (float)v[k] > 0.f ? 1 << k : 0;
+                        if (left < VEC) bits &= (1 << max(left, 0)) - 1;
+                        if (VEC == 4) bits |= __shfl_down(bits, 1) << 4;  // a byte is two lanes' four columns
+                        if ((VEC == 8 || !(c & 1)) && (n >> 3) < a.row_bytes) a.bits[(long)m * a.row_bytes + (n >> 3)] = (uint8_t)bits;
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
             }
         }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int r = lane / LANES; r < SIDE; r += 64 / LANES) {
-            const int c = (lane % LANES) * VEC;
-            const auto v = *reinterpret_cast<const typename Vec<T, VEC>::type *>(patch + r * PITCH + c * sizeof(T));
-            store_row<T>(a, m0 + wm * (TM / 4) + i * SIDE + r, n0 + wn * COLS + c, v);
-        }
-        __builtin_amdgcn_wave_barrier();
+        if (!more) break;
+        whole = whole && !a.bits;
+        now = next;
+        which ^= 1;
+        bid += gridDim.x;
+        more = place(bid + gridDim.x, next);
+        if (!more) next = now;
     }
+    dma_wait<0>();  // the repeated loads still write this workgroup's LDS
 }
 
 // Few rows: a workgroup takes 32 x 32 of Y and its eight waves an eighth of the blocks each, straight from memory to registers (no
@@ -350,17 +429,21 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(E4m3Args a) {
 
 template <int TM, int TN, class T>
 static int launch_tile(E4m3Args a, hipStream_t st) {
+    using Tile = E4m3Tile<TM, TN, T>;
     static PerDeviceOnce once;
     int dev;
-    constexpr int bytes = 4 * (TM + TN) * 64 + 4 * (TM + TN) * 4;
     if (once.pending(&dev)) {
-        if (hipFuncSetAttribute((const void *)linear_e4m3_kernel<TM, TN, T>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+        if (hipFuncSetAttribute((const void *)linear_e4m3_kernel<TM, TN, T>, hipFuncAttributeMaxDynamicSharedMemorySize, Tile::BYTES) !=
+            hipSuccess)
             return fail(PHONLP_ERR_LAUNCH, "linear_e4m3: hipFuncSetAttribute failed");
         once.mark(dev);
     }
     a.num_m = ceil_div(a.M, TM);
     a.num_n = ceil_div(a.N, TN);
-    hipLaunchKernelGGL((linear_e4m3_kernel<TM, TN, T>), dim3(tile_grid(a.num_m, a.num_n, 1)), dim3(512), bytes, st, a);
+    int grid = tile_grid(a.num_m, a.num_n, 1);
+    // one workgroup per compute unit; the loads look two blocks ahead, into the next tile alone, so a tile needs two
+    if (Tile::PERSIST && a.Kp >= 256 && grid > 256) grid = 256;
+    hipLaunchKernelGGL((linear_e4m3_kernel<TM, TN, T>), dim3(grid), dim3(512), Tile::BYTES, st, a);
     return check_launch("linear_e4m3_kernel");
 }
 
