@@ -58,23 +58,34 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, lon
     }
 }
 
-// ---- sorting, few tokens: a token's place is the number of (token, n) pairs before its own.  N^2 comparisons of which each is two
-// instructions, one launch.  A workgroup places 32 tokens, eight threads count an eighth of the others each.
+// ---- sorting, few tokens: a token's place is the number of (token, n) pairs before its own.  N^2 comparisons of two instructions
+// each, in one launch (8192 tokens: 4 us; a radix pass is two launches of 3 to 5).  A workgroup places 32 tokens, eight threads a token
+// count an eighth of the others each.
 template <class I>
 __global__ __launch_bounds__(256) void embedding_place_kernel(const I *tokens, int N, int V, int *order, int *sorted) {
-    __shared__ int keys[2048];
+    __shared__ __attribute__((aligned(16))) int keys[2048];
     __shared__ int counts[8][32];
-    const int own = threadIdx.x & 31, part = threadIdx.x >> 5, n = blockIdx.x * 32 + own;
+    const int own = threadIdx.x & 31, part = threadIdx.x >> 5, n0 = blockIdx.x * 32, n = n0 + own;
     const int key = n < N ? token_key(tokens, n, V) : 0;
     int count = 0;
     for (int base = 0; base < N; base += 2048) {
-        const int here = min(2048, N - base);
         __syncthreads();
-        for (int i = threadIdx.x; i < here; i += 256) keys[i] = token_key(tokens, base + i, V);
+        for (int i = threadIdx.x; i < 2048; i += 256) keys[i] = base + i < N ? token_key(tokens, base + i, V) : 0x7FFFFFFF;
         __syncthreads();
-        const int lo = part * 256, hi = min(lo + 256, here);
-        // before n equal tokens count too
-        for (int i = lo; i < hi; ++i) count += keys[i] < key + (base + i < n ? 1 : 0);
+        const int lo = part * 256;
+        if (base + lo >= N) continue;
+        // the 256 tokens of this thread: those before this workgroup's 32, those 32 (all in one thread's share, or none), those behind;
+        // equal ones count if they stand before n
+        const int split = min(max(n0 - base - lo, 0), 256), split32 = min(max(n0 + 32 - base - lo, 0), 256);
+        for (int i = 0; i < split; i += 4) {
+            const int4 k = *reinterpret_cast<const int4 *>(keys + lo + i);
+            count += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+        }
+        for (int i = split; i < split32; ++i) count += keys[lo + i] < key + (base + lo + i < n ? 1 : 0);
+        for (int i = split32; i < 256; i += 4) {
+            const int4 k = *reinterpret_cast<const int4 *>(keys + lo + i);
+            count += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
+        }
     }
     counts[part][own] = count;
     __syncthreads();
@@ -87,69 +98,57 @@ __global__ __launch_bounds__(256) void embedding_place_kernel(const I *tokens, i
     }
 }
 
-// ---- sorting, many tokens: stable radix passes of eight bits, tiles of 4096 pairs.
-constexpr int kSortTile = 4096;
-
+// ---- sorting, many tokens: stable radix passes of eight bits in at most 256 tiles of pairs, two launches a pass.
 template <class I>
 __device__ __forceinline__ int sort_key(const I *tokens, const int *keys, long n, int V) {
     return keys ? keys[n] : token_key(tokens, n, V);
 }
 
-// counts[digit][tile]
+// counts[tile][digit]
 template <class I>
-__global__ __launch_bounds__(256) void embedding_count_kernel(const I *tokens, const int *keys, int N, int V, int shift, int tiles, int *counts) {
+__global__ __launch_bounds__(256) void embedding_count_kernel(const I *tokens, const int *keys, int N, int V, int shift, int tile, int *counts) {
     __shared__ int bins[256];
     bins[threadIdx.x] = 0;
     __syncthreads();
-    const long base = (long)blockIdx.x * kSortTile;
-    for (int i = threadIdx.x; i < kSortTile && base + i < N; i += 256) atomicAdd(&bins[sort_key(tokens, keys, base + i, V) >> shift & 255], 1);
+    const long base = (long)blockIdx.x * tile;
+    for (int i = threadIdx.x; i < tile && base + i < N; i += 256) atomicAdd(&bins[sort_key(tokens, keys, base + i, V) >> shift & 255], 1);
     __syncthreads();
-    counts[(long)threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
-}
-
-// counts -> the number of pairs before (digit, tile), in place; one workgroup
-__global__ __launch_bounds__(1024) void embedding_scan_kernel(int *counts, int total) {
-    __shared__ int waves[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int carry = 0;
-    for (int base = 0; base < total; base += 1024) {
-        const int i = base + threadIdx.x;
-        const int v = i < total ? counts[i] : 0;
-        int s = v;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(s, d);
-            if (lane >= d) s += o;
-        }
-        if (lane == 63) waves[wave] = s;
-        __syncthreads();
-        int before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) {
-            before += w < wave ? waves[w] : 0;
-            all += waves[w];
-        }
-        if (i < total) counts[i] = carry + before + s - v;
-        carry += all;
-        __syncthreads();
-    }
+    counts[blockIdx.x * 256 + threadIdx.x] = bins[threadIdx.x];
 }
 
 template <class I>
 __global__ __launch_bounds__(256) void embedding_scatter_kernel(const I *tokens, const int *keys, const int *index, int N, int V, int shift,
-                                                                int tiles, const int *before, int *keys_out, int *index_out) {
+                                                                int tile, const int *counts, int *keys_out, int *index_out) {
     __shared__ int at[4][256];  // the next place of each wave's pairs of a digit
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long base = (long)blockIdx.x * kSortTile + wave * (kSortTile / 4);
+    __shared__ int totals[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tiles = gridDim.x;
+    const long base = (long)blockIdx.x * tile + wave * (tile / 4);
 #pragma unroll
     for (int w = 0; w < 4; ++w) at[w][threadIdx.x] = 0;
     __syncthreads();
-    for (int r = 0; r < kSortTile / 4; r += 64) {
+    for (int r = 0; r < tile / 4; r += 64) {
         const long n = base + r + lane;
         if (n < N) atomicAdd(&at[wave][sort_key(tokens, keys, n, V) >> shift & 255], 1);
     }
+    // this thread's digit: the pairs of smaller digits, and those of its own in the tiles before
+    int total = 0, before = 0;
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+        const int c = counts[t * 256 + threadIdx.x];
+        total += c;
+        before += t < (int)blockIdx.x ? c : 0;
+    }
+    int scan = total;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(scan, d);
+        if (lane >= d) scan += o;
+    }
+    if (lane == 63) totals[wave] = scan;
     __syncthreads();
-    int place = before[(long)threadIdx.x * tiles + blockIdx.x];
+    int place = before + scan - total;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) place += w < wave ? totals[w] : 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         const int c = at[w][threadIdx.x];
@@ -157,7 +156,7 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(const I *tokens,
         place += c;
     }
     __syncthreads();
-    for (int r = 0; r < kSortTile / 4; r += 64) {
+    for (int r = 0; r < tile / 4; r += 64) {
         const long n = base + r + lane;
         const bool in = n < N;
         const int key = in ? sort_key(tokens, keys, n, V) : 0, digit = key >> shift & 255;
@@ -229,55 +228,62 @@ struct SumArgs {
     float scale;
 };
 
-// blockIdx.y: a slab of 64 * VEC columns.  blockIdx.x < sum_blocks: a wave per chunk of R sorted places; behind them: a wave per 64
-// rows of the table, which writes zeros where no token points.
+// blockIdx.y: a slab of 64 * VEC columns.  blockIdx.x < sum_blocks: a wave per chunk of R sorted places, sixteen rows in flight; behind
+// them (first slab only): a wave per 16 rows of the table, which writes zeros where no token points.
 template <class T, class TO>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
-    constexpr int VEC = 16 / sizeof(T), UNROLL = 8;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = (blockIdx.y * 64 + lane) * VEC, left = a.E - col;
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 16;
+    typedef typename Vec<T, VEC>::type Vt;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TO *table = (TO *)a.d_table;
     if ((int)blockIdx.x >= a.sum_blocks) {
-        const long row0 = ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 64;
-        const long row = row0 + lane;
+        if (blockIdx.y) return;
+        const long row0 = ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 16, row = row0 + lane;
         bool empty = false;
-        if (row < a.V) {
+        if (lane < 16 && row < a.V) {
             const int at = lower_bound(a.sorted, 0, a.N, (int)row);
             empty = at == a.N || a.sorted[at] != (int)row;
         }
         unsigned long long rows = __ballot(empty);
-        const float zero[VEC] = {};
+        constexpr int VO = 16 / sizeof(TO);
+        const float zero[VO] = {};
         while (rows) {
             const int r = __ffsll(rows) - 1;
             rows &= rows - 1;
-            if (left > 0) store_row<TO, VEC>(table + (row0 + r) * a.E + col, left, zero, 0.f);
+            for (int c = lane * VO; c < a.E; c += 64 * VO) store_row<TO, VO>(table + (row0 + r) * a.E + c, a.E - c, zero, 0.f);
         }
         return;
     }
-    const int chunk = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
+    const int chunk = blockIdx.x * 4 + wave, col = (blockIdx.y * 64 + lane) * VEC, left = a.E - col;
     if (chunk >= a.chunks) return;
     const int first = chunk * a.R, last = min(first + a.R, a.N);
-    const T *d = (const T *)a.d_out;
-    const bool joined = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
-    bool head = joined;
+    const T *d = (const T *)a.d_out + col;
+    bool head = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
     float s[VEC] = {};
     for (int p = first; p < last; p += UNROLL) {
-        float v[UNROLL][VEC];
+        // lane u holds place p + u
+        const int at = p + lane, row = a.order[min(at, last - 1)], key = at < a.N ? a.sorted[at] : -1;
+        Vt v[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int q = min(p + u, last - 1);
-            if (left > 0) load_row<T, VEC>(d + (long)a.order[q] * a.ld + col, left, v[u]);
+            const T *q = d + (long)__builtin_amdgcn_readlane(row, u) * a.ld;
+            if (left >= VEC) {
+                v[u] = *reinterpret_cast<const Vt *>(q);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = i < left ? q[i] : (T)0.f;
+            }
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int q = p + u;
-            if (q >= last) break;
+            if (p + u >= last) break;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s[i] += v[u][i];
-            const int key = a.sorted[q];
-            const bool ends = q + 1 >= a.N || a.sorted[q + 1] != key;
-            if (!ends && q + 1 < last) continue;
-            if (left > 0 && key < a.V) {
-                if (ends && !head) store_row<TO, VEC>(table + (long)key * a.E + col, left, s, a.scale);
+            for (int i = 0; i < VEC; ++i) s[i] += (float)v[u][i];
+            const int k = __builtin_amdgcn_readlane(key, u);
+            const bool ends = __builtin_amdgcn_readlane(key, u + 1) != k;
+            if (!ends && p + u + 1 < last) continue;
+            if (left > 0 && k < a.V) {
+                if (ends && !head) store_row<TO, VEC>(table + (long)k * a.E + col, left, s, a.scale);
                 else store_row<float, VEC>(a.shares + ((long)chunk * 2 + (head ? 0 : 1)) * a.E + col, left, s, 1.f);
             }
             head = false;
@@ -287,48 +293,56 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
     }
 }
 
-// A wave per chunk whose last run begins in it and goes on behind it: the run's shares, in order.
+// A workgroup per chunk whose last run begins in it and goes on behind it: the run's shares, an eighth of them by each wave, in order.
 template <class T, class TO>
-__global__ __launch_bounds__(256) void embedding_join_kernel(SumArgs a) {
+__global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
     constexpr int VEC = 16 / sizeof(T), UNROLL = 8;
-    const int lane = threadIdx.x & 63, col = (blockIdx.y * 64 + lane) * VEC, left = a.E - col;
-    const int chunk = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (chunk >= a.chunks - 1) return;
+    __shared__ float sums[8][64 * VEC + 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = (blockIdx.y * 64 + lane) * VEC,
+              left = a.E - col, chunk = blockIdx.x;
     const int first = chunk * a.R, next = first + a.R, key = a.sorted[next - 1];
     if (key >= a.V || a.sorted[next] != key) return;
     if (a.sorted[first] == key && first > 0 && a.sorted[first - 1] == key) return;  // began before this chunk
     const int end = lower_bound(a.sorted, next, a.N, key + 1);
-    const int last = (end - 1) / a.R;  // the chunk of the run's last place
-    if (left <= 0) return;
-    float s[VEC];
-    load_row<float, VEC>(a.shares + ((long)chunk * 2 + 1) * a.E + col, left, s);
-    for (int c = chunk + 1; c <= last; c += UNROLL) {
-        float v[UNROLL][VEC];
+    // shares 0 .. count: this chunk's last run, then the first run of each chunk to the one of the run's last place
+    const int count = (end - 1) / a.R - chunk, per = ceil_div(count + 1, 8), lo = wave * per, hi = min(lo + per, count + 1);
+    float s[VEC] = {};
+    if (left > 0)
+        for (int c = lo; c < hi; c += UNROLL) {
+            float v[UNROLL][VEC];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) load_row<float, VEC>(a.shares + (long)min(c + u, last) * 2 * a.E + col, left, v[u]);
+            for (int u = 0; u < UNROLL; ++u) {
+                const int k = min(c + u, hi - 1);
+                load_row<float, VEC>(a.shares + ((long)(chunk + k) * 2 + (k ? 0 : 1)) * a.E + col, left, v[u]);
+            }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+            for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (c + u <= last) s[i] += v[u][i];
-    }
+                for (int i = 0; i < VEC; ++i)
+                    if (c + u < hi) s[i] += v[u][i];
+        }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[wave][lane * VEC + i] = s[i];
+    __syncthreads();
+    if (wave || left <= 0) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] += sums[w][lane * VEC + i];
     store_row<TO, VEC>((TO *)a.d_table + (long)key * a.E + col, left, s, a.scale);
 }
 
-constexpr int kPlaceMost = 16384;
-static int sum_places(int N) {  // sorted places of one wave: few enough to fill the chip, few enough chunks to join
-    int R = ceil_div(ceil_div(N, 2048), 32) * 32;
-    return R;
-}
+constexpr int kPlaceMost = 8192;
 struct EmbeddingPlan {
-    int R, chunks, tiles;
+    int R, chunks, tile, tiles;  // places of one wave; pairs of a sorting tile
     size_t pairs, shares, counts, total;
 };
 static EmbeddingPlan plan_embedding(int N, int E) {
     EmbeddingPlan p;
-    p.R = sum_places(N);
+    p.R = ceil_div(ceil_div(N, 4096), 16) * 16;  // enough waves to fill the chip, few enough shares to join
     p.chunks = ceil_div(N, p.R);
-    p.tiles = ceil_div(N, kSortTile);
+    p.tile = ceil_div(ceil_div(N, 256), 1024) * 1024;
+    p.tiles = ceil_div(N, p.tile);
     p.pairs = align_up((size_t)N * 4, 256);
     p.shares = align_up((size_t)p.chunks * 2 * E * 4, 256);
     const bool radix = N > kPlaceMost;
@@ -352,10 +366,9 @@ static int sort_tokens(const I *tokens, int N, int V, const EmbeddingPlan &pl, c
     const int *from_keys = nullptr, *from_index = nullptr;
     int now = 0;
     for (int shift = 0; shift == 0 || (shift < 31 && (V >> shift) > 0); shift += 8, now ^= 1) {  // keys 0 .. V
-        hipLaunchKernelGGL((embedding_count_kernel<I>), dim3(pl.tiles), dim3(256), 0, st, tokens, from_keys, N, V, shift, pl.tiles, counts);
-        hipLaunchKernelGGL(embedding_scan_kernel, dim3(1), dim3(1024), 0, st, counts, pl.tiles * 256);
+        hipLaunchKernelGGL((embedding_count_kernel<I>), dim3(pl.tiles), dim3(256), 0, st, tokens, from_keys, N, V, shift, pl.tile, counts);
         hipLaunchKernelGGL((embedding_scatter_kernel<I>), dim3(pl.tiles), dim3(256), 0, st, tokens, from_keys, from_index, N, V, shift,
-                           pl.tiles, counts, keys[now], index[now]);
+                           pl.tile, counts, keys[now], index[now]);
         const int rc = check_launch("embedding_scatter_kernel");
         if (rc) return rc;
         from_keys = keys[now];
@@ -373,12 +386,12 @@ static int sum_rows(SumArgs a, hipStream_t st) {
     a.sum_blocks = ceil_div(a.chunks, 4);
     {
         ProfScope ps("embedding_sum", st);
-        hipLaunchKernelGGL((embedding_sum_kernel<T, TO>), dim3(a.sum_blocks + ceil_div(a.V, 256), slabs), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((embedding_sum_kernel<T, TO>), dim3(a.sum_blocks + ceil_div(a.V, 64), slabs), dim3(256), 0, st, a);
         const int rc = check_launch("embedding_sum_kernel");
         if (rc || a.chunks == 1) return rc;
     }
     ProfScope ps("embedding_join", st);
-    hipLaunchKernelGGL((embedding_join_kernel<T, TO>), dim3(ceil_div(a.chunks - 1, 4), slabs), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((embedding_join_kernel<T, TO>), dim3(a.chunks - 1, slabs), dim3(512), 0, st, a);
     return check_launch("embedding_join_kernel");
 }
 

@@ -35,7 +35,7 @@ def _tokens(g, N, V, spread):
 # one token; one row; fewer tokens than a chunk; runs over many chunks; the border between the two sorts and both sides of it;
 # more than one radix pass; odd and one-column rows; more slabs than one
 CASES = [(1, 1, 1, "even"), (1, 64000, 768, "even"), (37, 24, 100, "zipf"), (31, 7, 3, "outside"), (2000, 24, 100, "zipf"),
-         (4000, 3, 130, "one"), (5000, 5000, 33, "even"), (16384, 300, 17, "zipf"), (16385, 300, 17, "zipf"), (20000, 70000, 8, "zipf"),
+         (4000, 3, 130, "one"), (5000, 5000, 33, "even"), (8192, 300, 17, "zipf"), (8193, 300, 17, "zipf"), (16385, 300, 17, "zipf"), (300001, 40, 9, "zipf"), (20000, 70000, 8, "zipf"),
          (40000, 24, 100, "zipf"), (33000, 200, 257, "one"), (17000, 1000, 1100, "outside"), (90001, 65536, 5, "even")]
 
 
