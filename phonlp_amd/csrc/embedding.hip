@@ -15,46 +15,38 @@ __device__ __forceinline__ int token_key(const I *tokens, long n, int V) {  // V
     return t >= 0 && t < (I)V ? (int)t : V;
 }
 
+// A wave takes sixteen tokens and a slab of 64 * VEC columns (blockIdx.y): one load for the tokens, a lane each, sixteen rows in flight.
+// Lanes behind a row's end stay with the others: the tokens are read from all sixteen lanes.
 template <class T, class I>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, long ld, const I *tokens, int N, int V, int E, float scale,
                                                              T *out) {
-    constexpr int VEC = 16 / sizeof(T), UNROLL = 4;
+    constexpr int VEC = 16 / sizeof(T), ROWS = 16;
     typedef typename Vec<T, VEC>::type Vt;
-    const int per_row = (E + VEC - 1) / VEC;
-    const long total = (long)N * per_row, step = (long)gridDim.x * 256;
-    for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < total; g += step * UNROLL) {
-        Vt v[UNROLL];
-        long at[UNROLL];
-        int left[UNROLL];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = (blockIdx.y * 64 + lane) * VEC,
+              left = E - col;
+    const long n0 = (blockIdx.x * 4L + wave) * ROWS;
+    if (n0 >= N) return;  // the whole wave
+    const int rows = (int)min((long)ROWS, N - n0), held = token_key(tokens, n0 + min(lane, rows - 1), V);
+    int key[ROWS];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const long it = g + u * step;
-            left[u] = 0;
-            if (it >= total) continue;
-            const long n = total < (1L << 31) ? (long)((unsigned)it / (unsigned)per_row) : it / per_row;
-            const int c = (int)(it - n * per_row) * VEC, key = token_key(tokens, n, V);
-            at[u] = n * E + c;
-            left[u] = min(E - c, VEC);
-            const T *p = table + key * ld + c;
-            if (key < V && left[u] == VEC) {
-                v[u] = *reinterpret_cast<const Vt *>(p);
-            } else {
+    for (int u = 0; u < ROWS; ++u) key[u] = __builtin_amdgcn_readlane(held, u);
+    if (left >= VEC) {
+        Vt v[ROWS];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[u][i] = key < V && i < left[u] ? p[i] : (T)0.f;
-            }
+        for (int u = 0; u < ROWS; ++u) v[u] = *reinterpret_cast<const Vt *>(table + (key[u] < V ? key[u] : 0) * ld + col);
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+            Vt o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] = key[u] < V ? (T)((float)v[u][i] * scale) : (T)0.f;
+            if (u < rows) *reinterpret_cast<Vt *>(out + (n0 + u) * E + col) = o;
         }
+    } else if (left > 0) {  // the one lane at a row's end that has less than VEC columns
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[u][i] = (T)((float)v[u][i] * scale);
-            if (left[u] == VEC) {
-                *reinterpret_cast<Vt *>(out + at[u]) = v[u];
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    if (i < left[u]) out[at[u] + i] = v[u][i];
-            }
-        }
+        for (int u = 0; u < ROWS; ++u)
+            if (u < rows)
+                for (int i = 0; i < left; ++i)
+                    out[(n0 + u) * E + col + i] = key[u] < V ? (T)((float)table[key[u] * ld + col + i] * scale) : (T)0.f;
     }
 }
 
@@ -70,19 +62,21 @@ __global__ __launch_bounds__(256) void embedding_place_kernel(const I *tokens, i
     int count = 0;
     for (int base = 0; base < N; base += 2048) {
         __syncthreads();
-        for (int i = threadIdx.x; i < 2048; i += 256) keys[i] = base + i < N ? token_key(tokens, base + i, V) : 0x7FFFFFFF;
+        for (int i = threadIdx.x; i < min(2048, N - base + 4); i += 256)
+            if (i < 2048) keys[i] = base + i < N ? token_key(tokens, base + i, V) : 0x7FFFFFFF;
         __syncthreads();
         const int lo = part * 256;
         if (base + lo >= N) continue;
-        // the 256 tokens of this thread: those before this workgroup's 32, those 32 (all in one thread's share, or none), those behind;
+        // up to 256 tokens of this thread: those before this workgroup's 32, those 32 (all in one thread's share, or none), those behind;
         // equal ones count if they stand before n
-        const int split = min(max(n0 - base - lo, 0), 256), split32 = min(max(n0 + 32 - base - lo, 0), 256);
+        const int mine = min((N - base - lo + 3) & ~3, 256), split = min(max(n0 - base - lo, 0), mine),
+                  split32 = min(max(n0 + 32 - base - lo, 0), mine);
         for (int i = 0; i < split; i += 4) {
             const int4 k = *reinterpret_cast<const int4 *>(keys + lo + i);
             count += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
         }
         for (int i = split; i < split32; ++i) count += keys[lo + i] < key + (base + lo + i < n ? 1 : 0);
-        for (int i = split32; i < 256; i += 4) {
+        for (int i = split32; i < mine; i += 4) {
             const int4 k = *reinterpret_cast<const int4 *>(keys + lo + i);
             count += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
         }
@@ -293,21 +287,29 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
     }
 }
 
-// A workgroup per chunk whose last run begins in it and goes on behind it: the run's shares, an eighth of them by each wave, in order.
+// Runs that go on behind the chunk they begin in: their shares, in order.  A workgroup looks at eight chunks, a chunk per lane; runs of
+// up to 17 shares are summed by a wave each, longer ones by all eight waves, an eighth of the shares each.
 template <class T, class TO>
 __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
-    constexpr int VEC = 16 / sizeof(T), UNROLL = 8;
-    __shared__ float sums[8][64 * VEC + 4];
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 16 / (VEC / 4), FEW = 16;
+    __shared__ float sums[8][64 * VEC];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = (blockIdx.y * 64 + lane) * VEC,
-              left = a.E - col, chunk = blockIdx.x;
-    const int first = chunk * a.R, next = first + a.R, key = a.sorted[next - 1];
-    if (key >= a.V || a.sorted[next] != key) return;
-    if (a.sorted[first] == key && first > 0 && a.sorted[first - 1] == key) return;  // began before this chunk
-    const int end = lower_bound(a.sorted, next, a.N, key + 1);
-    // shares 0 .. count: this chunk's last run, then the first run of each chunk to the one of the run's last place
-    const int count = (end - 1) / a.R - chunk, per = ceil_div(count + 1, 8), lo = wave * per, hi = min(lo + per, count + 1);
-    float s[VEC] = {};
-    if (left > 0)
+              left = a.E - col, mine = blockIdx.x * 8 + lane;
+    auto reaches = [&](int chunk, int k) {  // the first place of `chunk` still holds k
+        const long p = (long)chunk * a.R;
+        return (p < a.N) & (a.sorted[min(p, (long)a.N - 1)] == k);
+    };
+    int key = a.V, count = 1;  // shares behind the chunk's own, at most FEW
+    if (lane < 8 && mine < a.chunks - 1) {
+        const int first = mine * a.R, k = a.sorted[first + a.R - 1];
+        const bool began_before = a.sorted[first] == k && first > 0 && a.sorted[first - 1] == k;
+        if (k < a.V && reaches(mine + 1, k) && !began_before) {
+            key = k;
+#pragma unroll
+            for (int i = 2; i <= FEW; ++i) count += reaches(mine + i, k);
+        }
+    }
+    auto add = [&](int chunk, int lo, int hi, float (&s)[VEC]) {  // shares lo .. hi - 1: the chunk's last run, then the next chunks' first
         for (int c = lo; c < hi; c += UNROLL) {
             float v[UNROLL][VEC];
 #pragma unroll
@@ -321,15 +323,37 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
                 for (int i = 0; i < VEC; ++i)
                     if (c + u < hi) s[i] += v[u][i];
         }
+    };
+    int turn = 0;
+    for (unsigned long long runs = __ballot(key < a.V); runs; runs &= runs - 1) {
+        const int l = __ffsll(runs) - 1, chunk = blockIdx.x * 8 + l, k = __builtin_amdgcn_readlane(key, l);
+        int n = __builtin_amdgcn_readlane(count, l) + 1;
+        if (n > FEW) {  // how many of the chunks left it reaches: 64 of them far apart, then the 64 (or more) in between, and so on
+            for (int apart = ceil_div(a.chunks - chunk - n, 64); apart > 0; apart = apart > 1 ? ceil_div(apart, 64) : 0)
+                n += __popcll(__ballot(reaches(chunk + n + lane * apart + apart - 1, k))) * apart;
+        }
+        float s[VEC] = {};
+        if (n <= FEW + 1) {
+            if ((turn++ & 7) == wave && left > 0) {
+                add(chunk, 0, n, s);
+                store_row<TO, VEC>((TO *)a.d_table + (long)k * a.E + col, left, s, a.scale);
+            }
+            continue;
+        }
+        const int per = ceil_div(n, 8);
+        if (left > 0) add(chunk, wave * per, min(wave * per + per, n), s);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sums[wave][lane * VEC + i] = s[i];
-    __syncthreads();
-    if (wave || left <= 0) return;
+        for (int i = 0; i < VEC; ++i) sums[wave][i * 64 + lane] = s[i];
+        __syncthreads();
+        if (wave == 0 && left > 0) {
 #pragma unroll
-    for (int w = 1; w < 8; ++w)
+            for (int w = 1; w < 8; ++w)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[i] += sums[w][lane * VEC + i];
-    store_row<TO, VEC>((TO *)a.d_table + (long)key * a.E + col, left, s, a.scale);
+                for (int i = 0; i < VEC; ++i) s[i] += sums[w][i * 64 + lane];
+            store_row<TO, VEC>((TO *)a.d_table + (long)k * a.E + col, left, s, a.scale);
+        }
+        __syncthreads();
+    }
 }
 
 constexpr int kPlaceMost = 8192;
@@ -391,7 +415,7 @@ static int sum_rows(SumArgs a, hipStream_t st) {
         if (rc || a.chunks == 1) return rc;
     }
     ProfScope ps("embedding_join", st);
-    hipLaunchKernelGGL((embedding_join_kernel<T, TO>), dim3(a.chunks - 1, slabs), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((embedding_join_kernel<T, TO>), dim3(ceil_div(a.chunks - 1, 8), slabs), dim3(512), 0, st, a);
     return check_launch("embedding_join_kernel");
 }
 
@@ -401,7 +425,8 @@ using namespace phonlp;
 
 extern "C" int phonlp_embedding_rows(const void *table, int type, long ld, const void *tokens, int tokens_are_int64, int N, int V, int E,
                                      float scale, void *out, void *stream) {
-    if (!table || !tokens || !out || !type_ok(type) || N <= 0 || V <= 0 || E <= 0 || ld < E || V == 0x7FFFFFFF)
+    if (!table || !tokens || !out || !type_ok(type) || N <= 0 || N > (1 << 30) || V <= 0 || E <= 0 || E > (1 << 22) || ld < E ||
+        V == 0x7FFFFFFF)
         return fail(PHONLP_ERR_SHAPE, "embedding_rows: bad argument");
     if ((uintptr_t)table % type_bytes(type) || (uintptr_t)out % type_bytes(type) || (uintptr_t)tokens % (tokens_are_int64 ? 8 : 4))
         return fail(PHONLP_ERR_SHAPE, "embedding_rows: table, tokens and out must have their types' alignment");
@@ -410,8 +435,7 @@ extern "C" int phonlp_embedding_rows(const void *table, int type, long ld, const
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         constexpr int VEC = 16 / sizeof(T);
-        const long blocks = ((long)N * ceil_div(E, VEC) + 255) / 256;
-        const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+        const dim3 grid(ceil_div(ceil_div(N, 16), 4), ceil_div(E, 64 * VEC));
         if (tokens_are_int64)
             hipLaunchKernelGGL((embedding_rows_kernel<T, long>), grid, dim3(256), 0, st, (const T *)table, ld, (const long *)tokens, N, V, E,
                                scale, (T *)out);
