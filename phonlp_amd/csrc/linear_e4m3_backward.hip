@@ -41,25 +41,25 @@ struct BwPrep {
     long lddy;
     const uint32_t *bits;
     uint16_t *planes;  // [P][Mp][Np]
-    float *part;       // column sums of 128 rows, [blocks of rows][N]
+    float *part;       // column sums of dz_rows rows, [blocks of rows][N]
     const uint8_t *codes[2], *exps[2];  // images of x and w
     __bf16 *wide[2];                    // their values, [rows up to a multiple of 32][Kp]
     int rows[2], wide_blocks[2];
-    int words, M, N, Mp, Np, Kp, KB4, dz_m, dz_blocks;
+    int words, M, N, Mp, Np, Kp, KB4, dz_rows, dz_m, dz_blocks;  // dz_rows: rows of a workgroup
 };
 
-// dY -> the pieces of dZ (zero behind M and N) and the column sums.  A workgroup takes 128 rows x 256 columns, a thread eight columns
+// dY -> the pieces of dZ (zero behind M and N) and the column sums.  A workgroup takes dz_rows x 256 columns, a thread eight columns
 // of every eighth row; the eight threads of a column group add in order.
 template <class T>
 __device__ __forceinline__ void prep_dz(const BwPrep &a, int bid, float (&sums)[8][256]) {
     constexpr int P = Pieces<T>::N;
     typedef typename Vec<T, 8>::type V;
     const int bm = bid % a.dz_m, bn = bid / a.dz_m;
-    const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5, n = bn * 256 + cg * 8, m0 = bm * 128 + rl;
+    const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5, n = bn * 256 + cg * 8, m0 = bm * a.dz_rows + rl;
     float s[8] = {};
     if (n < a.Np) {
 #pragma unroll 4
-        for (int it = 0; it < 16; ++it) {
+        for (int it = 0; it < a.dz_rows / 8; ++it) {
             const int m = m0 + it * 8;
             if (m >= a.Mp) break;
             float v[8];
@@ -369,11 +369,18 @@ __device__ __forceinline__ void bw_join(const BwJoin &q, int bid) {
     for (long at = (bid * 256L + threadIdx.x) * 4; at < q.total; at += q.blocks * 1024L) {
         const int left = (int)min(q.total - at, 4L);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < q.S; ++s) {
-            const float *p = q.part + s * q.total + at;
-            if (left == 4) v += *reinterpret_cast<const Vec<float, 4>::type *>(p);
-            else
-                for (int i = 0; i < left; ++i) v[i] += p[i];
+        if (left == 4) {
+            for (int s = 0; s < q.S; s += 8) {  // eight loads in flight
+                f32x4 p[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) p[u] = *reinterpret_cast<const Vec<float, 4>::type *>(q.part + min(s + u, q.S - 1) * q.total + at);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (s + u < q.S) v += p[u];
+            }
+        } else {
+            for (int s = 0; s < q.S; ++s)
+                for (int i = 0; i < left; ++i) v[i] += q.part[s * q.total + at + i];
         }
         store_quad((T *)q.out + at, v, left);
     }
@@ -396,13 +403,20 @@ struct BwPlan {
     Split sx, sw;
     size_t planes, part, wx, ww, px, pw, total;
 };
+// Rows of a workgroup that makes dZ: enough workgroups to fill the chip, few enough partial sums.
+static int dz_rows_of(int M, int N) {
+    const long blocks = (long)ceil_div(M, 128) * ceil_div(N, 256);
+    return blocks >= 1024 ? 128 : blocks >= 512 ? 64 : 32;
+}
 static double plan_split(int I, int J, int R, int P, int TI, int TJ, Split *out) {
     const double tiles = (double)ceil_div(I, TI) * ceil_div(J, TJ), part = (TI * TJ) / (256. * 256.) * 0.65 + 0.1;  // us of a part
-    const int steps = ceil_div(R, 32);
+    const int steps = ceil_div(R, 32), fill = tiles < 256 ? (int)(256 / tiles) : 1;
     double least = 1e300;
-    for (int S = 1; S <= 64 && S <= steps; ++S) {
+    const int tries[] = {1, fill / 2, fill, 2 * fill};
+    for (int S : tries) {
+        S = S < 1 ? 1 : S > 64 ? 64 : S > steps ? steps : S;
         const int per = ceil_div(steps, S);
-        if (ceil_div(steps, per) != S) continue;
+        S = ceil_div(steps, per);
         const double one = per * P * part + 4.0, rounds = tiles * S / 256.;
         // the last round is rarely full: a share of a workgroup's time on top
         const double us = (rounds > 1. ? (rounds + 0.4) : 1.) * one + (S > 1 ? 4.0 + 8.0 * S * I * (double)J / 4.0e6 : 0.0);
@@ -413,15 +427,14 @@ static double plan_split(int I, int J, int R, int P, int TI, int TJ, Split *out)
     }
     return least;
 }
-static BwPlan plan_bw(int M, int N, int K, int type, bool need_x, bool need_w) {
+static BwPlan plan_bw(int M, int N, int K, int type) {
     const int P = pieces_of(type);
     BwPlan p = {};
     double least = 1e300;
     for (int IF = 4; IF >= 2; IF -= 2)
         for (int JF = 8; JF >= 4; JF -= JF == 6 ? 2 : 1) {
-            Split sx = {1, 1}, sw = {1, 1};
-            const double us = (need_x ? plan_split(M, K, N, P, IF * 64, JF * 32, &sx) : 0.) +
-                              (need_w ? plan_split(N, K, M, P, IF * 64, JF * 32, &sw) : 0.);
+            Split sx, sw;
+            const double us = plan_split(M, K, N, P, IF * 64, JF * 32, &sx) + plan_split(N, K, M, P, IF * 64, JF * 32, &sw);
             if (us < least) {
                 least = us;
                 p.IF = IF;
@@ -432,9 +445,9 @@ static BwPlan plan_bw(int M, int N, int K, int type, bool need_x, bool need_w) {
         }
     const size_t Kp = kp8_of(K);
     p.planes = align_up((size_t)P * up_to(M, 32) * up_to(N, 32) * 2, 256);
-    p.part = align_up((size_t)ceil_div(M, 128) * N * 4, 256);
-    p.wx = need_w ? up_to(M, 32) * Kp * 2 : 0;
-    p.ww = need_x ? up_to(N, 32) * Kp * 2 : 0;
+    p.part = align_up((size_t)ceil_div(M, dz_rows_of(M, N)) * N * 4, 256);
+    p.wx = up_to(M, 32) * Kp * 2;
+    p.ww = up_to(N, 32) * Kp * 2;
     p.px = p.sx.S > 1 ? align_up((size_t)p.sx.S * M * K * 4, 256) : 0;
     p.pw = p.sw.S > 1 ? align_up((size_t)p.sw.S * N * K * 4, 256) : 0;
     p.total = p.planes + p.part + p.wx + p.ww + p.px + p.pw;
@@ -473,13 +486,7 @@ static bool bw_shape_ok(int M, int N, int K, int type) {
 }
 
 extern "C" size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int type) {
-    if (!bw_shape_ok(M, N, K, type)) return 0;
-    size_t most = 0;  // whichever of dX and dW is asked for
-    for (int need = 1; need < 4; ++need) {
-        const size_t total = plan_bw(M, N, K, type, need & 1, need & 2).total;
-        most = total > most ? total : most;
-    }
-    return most;
+    return bw_shape_ok(M, N, K, type) ? plan_bw(M, N, K, type).total : 0;
 }
 
 extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, const uint32_t *bits, const void *x_codes,
@@ -491,12 +498,12 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
         ((uintptr_t)bits & 3) || ((uintptr_t)dw & 3) || ((uintptr_t)db & 3) || (uintptr_t)dy % type_bytes(type) ||
         (uintptr_t)dx % type_bytes(type))
         return fail(PHONLP_ERR_SHAPE, "linear_e4m3_backward: codes must be 16-byte aligned, exponents, bits, dw and db 4-byte, dy and dx to their type");
-    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < phonlp_linear_e4m3_backward_ws_bytes(M, N, K, type))
+    const BwPlan pl = plan_bw(M, N, K, type);
+    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < pl.total)
         return fail(PHONLP_ERR_WORKSPACE, "linear_e4m3_backward: workspace too small or not 16-byte aligned");
     if (!dx && !dw && !db) return PHONLP_OK;
     hipStream_t st = as_stream(stream);
-    const BwPlan pl = plan_bw(M, N, K, type, dx, dw);
-    const int Mp = up_to(M, 32), Np = up_to(N, 32), Kp = kp8_of(K), parts = ceil_div(M, 128);
+    const int Mp = up_to(M, 32), Np = up_to(N, 32), Kp = kp8_of(K), dz_rows = dz_rows_of(M, N), parts = ceil_div(M, dz_rows);
     uint8_t *planes = (uint8_t *)ws, *p = planes + pl.planes;
     float *part = (float *)p;
     uint8_t *wx = p + pl.part, *ww = wx + pl.wx;
@@ -506,7 +513,7 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
     const bool make_planes = (dx || dw) && !direct;
     BwPrep prep = {dy, lddy, bits, make_planes ? (uint16_t *)planes : nullptr, !db ? nullptr : parts == 1 ? db : part,
                    {(const uint8_t *)x_codes, (const uint8_t *)w_codes}, {x_exponents, w_exponents}, {(__bf16 *)wx, (__bf16 *)ww}, {M, N},
-                   {0, 0}, ceil_div(N, 32), M, N, Mp, Np, Kp, kb4_of(K), ceil_div(Mp, 128), 0};
+                   {0, 0}, ceil_div(N, 32), M, N, Mp, Np, Kp, kb4_of(K), dz_rows, ceil_div(Mp, dz_rows), 0};
     if (make_planes || db) prep.dz_blocks = prep.dz_m * ceil_div(Np, 256);
     auto wide_blocks = [&](int rows) {
         const long blocks = ((long)up_to(rows, 32) * (Kp / 16) + 1023) / 1024;
@@ -554,7 +561,7 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
         if (!jx && !jw) return PHONLP_OK;
         ProfScope ps("e4m3_bw_join", st);
         auto plan = [](bool on, const float *p, void *out, long total, int S) {
-            const long blocks = on ? (total + 1023) / 1024 : 0;
+            const long blocks = on ? (total + 1023) / 1024 : 0;  // four values a thread and turn
             return BwJoin{p, out, total, S, (int)(blocks < 2048 ? blocks : 2048)};
         };
         const BwJoin x = plan(jx, px, dx, (long)M * K, pl.sx.S), w = plan(jw, pw, dw, (long)N * K, pl.sw.S);

@@ -968,19 +968,25 @@ def _run(device, name, *args):
         check(rc, name)
 
 
+def _new(rows: int, cols: int, dtype, device) -> Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)  # a quarter less host time than torch.empty
+
+
 def _rows_of(t: Tensor, name: str):
-    """A 2-d device tensor of fp32 / bf16 / fp16 rows with unit column stride -> (type code, row pitch)."""
+    """A 2-d device tensor of fp32 / bf16 / fp16 rows with unit column stride -> (type code, row pitch, rows, columns)."""
     code = _TYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name}: expected dtype float32, bfloat16 or float16, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a ROCm device tensor (phonlp_amd has no CPU path)")
-    if t.dim() != 2:
-        raise ValueError(f"{name}: expected 2 dimensions, got {t.dim()}")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name}: expected 2 dimensions, got {len(shape)}")
+    rows, cols = shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1 or rows > 1 and ld < cols:
         raise ValueError(f"{name}: expected rows of unit column stride that do not overlap (pass .contiguous())")
-    return code, max(t.stride(0), cols) if rows > 1 else cols
+    return code, ld if rows > 1 else cols, rows, cols
 
 
 def _same_device(device, **tensors):
@@ -1005,27 +1011,27 @@ def _image_of(codes: Tensor, exponents: Tensor, K: int, name: str) -> int:
         raise ValueError(f"{name}: expected float8_e4m3fn codes and uint8 exponents, got {codes.dtype} and {exponents.dtype}")
     if not codes.is_cuda:
         raise ValueError(f"{name}: expected a ROCm device tensor (phonlp_amd has no CPU path)")
-    if K < 1 or codes.dim() != 2 or codes.shape[1] != e4m3_kp(K) or tuple(exponents.shape) != (codes.shape[0], e4m3_kb(K)):
+    shape = codes.shape
+    if K < 1 or len(shape) != 2 or shape[1] != -(-K // 128) * 128 or exponents.shape != (shape[0], -(-K // 512) * 4):
         raise ValueError(f"{name}: expected codes [rows, {e4m3_kp(K)}] and exponents [rows, {e4m3_kb(K)}] for K = {K}, "
-                         f"got {tuple(codes.shape)} and {tuple(exponents.shape)}")
+                         f"got {tuple(shape)} and {tuple(exponents.shape)}")
     if not (codes.is_contiguous() and exponents.is_contiguous()):
         raise ValueError(f"{name}: expected contiguous tensors")
     if exponents.device != codes.device:
         raise ValueError(f"{name}: codes and exponents are on different devices")
-    return codes.shape[0]
+    return shape[0]
 
 
 def e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
     """x [rows, K] fp32 / bf16 / fp16 (row stride free, unit column stride) -> its e4m3 image: codes float8_e4m3fn
     [rows, e4m3_kp(K)], exponents uint8 [rows, e4m3_kb(K)] (one power-of-two scale per row and block of 128 columns; infinities and
     NaN become NaN).  The operand form of linear_e4m3, and a layer input's 8-bit checkpoint for linear_e4m3_backward."""
-    code, ld = _rows_of(x, "x")
-    rows, K = x.shape
+    code, ld, rows, K = _rows_of(x, "x")
     if K == 0:
         raise ValueError("e4m3_rows: x has no columns")
     dev = x.device
-    codes = torch.empty((rows, e4m3_kp(K)), dtype=_E4M3, device=dev)
-    exponents = torch.empty((rows, e4m3_kb(K)), dtype=torch.uint8, device=dev)
+    codes = _new(rows, -(-K // 128) * 128, _E4M3, dev)
+    exponents = _new(rows, -(-K // 512) * 4, torch.uint8, dev)
     if rows:
         _run(dev, "phonlp_e4m3_rows", x.data_ptr(), code, ld, rows, K, codes.data_ptr(), exponents.data_ptr())
     return codes, exponents
@@ -1037,7 +1043,7 @@ def e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype = t
     if dtype not in _TYPES:
         raise ValueError(f"e4m3_values: dtype must be float32, bfloat16 or float16, got {dtype}")
     dev = codes.device
-    out = torch.empty((rows, K), dtype=dtype, device=dev)
+    out = _new(rows, K, dtype, dev)
     if rows:
         _run(dev, "phonlp_e4m3_values", codes.data_ptr(), exponents.data_ptr(), rows, K, _TYPES[dtype], out.data_ptr())
     return out
@@ -1056,8 +1062,8 @@ def linear_e4m3(x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponen
         raise ValueError(f"bias: expected a contiguous float32 tensor [{N}], got {bias.dtype} {tuple(bias.shape)}")
     if dtype not in _TYPES:
         raise ValueError(f"linear_e4m3: dtype must be float32, bfloat16 or float16, got {dtype}")
-    y = torch.empty((M, N), dtype=dtype, device=dev)
-    bits = torch.empty((M, (N + 31) // 32), dtype=torch.int32, device=dev) if want_bits else None
+    y = _new(M, N, dtype, dev)
+    bits = _new(M, (N + 31) // 32, torch.int32, dev) if want_bits else None
     if M and N:
         _run(dev, "phonlp_linear_e4m3", x_codes.data_ptr(), x_exponents.data_ptr(), w_codes.data_ptr(), w_exponents.data_ptr(),
              None if bias is None else bias.data_ptr(), y.data_ptr(), _TYPES[dtype], None if bits is None else bits.data_ptr(), M, N, K,
@@ -1070,22 +1076,22 @@ def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_
     """Backward of linear_e4m3 from the checkpoint: dY [M, N] fp32 / bf16 / fp16 (row stride free), bits of a ReLU layer (None: no
     ReLU), the images of the layer's input and weight -> (dX [M, K] of dY's type, dW [N, K] fp32, db [N] fp32), None where not asked
     for.  The quantisation of x and w counts as the identity."""
-    code, ld = _rows_of(dY, "dY")
+    code, ld, *shape = _rows_of(dY, "dY")
     M = _image_of(x_codes, x_exponents, K, "x_codes")
     N = _image_of(w_codes, w_exponents, K, "w_codes")
     dev = dY.device
     _same_device(dev, x_codes=x_codes, w_codes=w_codes, bits=bits)
-    if tuple(dY.shape) != (M, N):
-        raise ValueError(f"dY: expected [{M}, {N}] by the images, got {tuple(dY.shape)}")
+    if shape != [M, N]:
+        raise ValueError(f"dY: expected [{M}, {N}] by the images, got {shape}")
     if bits is not None and (bits.dtype != torch.int32 or tuple(bits.shape) != (M, (N + 31) // 32) or not bits.is_contiguous()):
         raise ValueError(f"bits: expected a contiguous int32 tensor [{M}, {(N + 31) // 32}], got {bits.dtype} {tuple(bits.shape)}")
     if M == 0 or N == 0:  # empty sums
         zeros = lambda *shape, t: torch.zeros(shape, dtype=t, device=dev)
         return (zeros(M, K, t=dY.dtype) if need_dX else None, zeros(N, K, t=torch.float32) if need_dW else None,
                 zeros(N, t=torch.float32) if need_db else None)
-    dX = torch.empty((M, K), dtype=dY.dtype, device=dev) if need_dX else None
-    dW = torch.empty((N, K), dtype=torch.float32, device=dev) if need_dW else None
-    db = torch.empty((N,), dtype=torch.float32, device=dev) if need_db else None
+    dX = _new(M, K, dY.dtype, dev) if need_dX else None
+    dW = _new(N, K, torch.float32, dev) if need_dW else None
+    db = torch.empty_strided((N,), (1,), dtype=torch.float32, device=dev) if need_db else None
     if not (need_dX or need_dW or need_db):
         return None, None, None
     nb = lib().phonlp_linear_e4m3_backward_ws_bytes(M, N, K, code)
@@ -1106,9 +1112,8 @@ def _tokens_of(tokens: Tensor, device) -> int:
 def embedding_rows(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
     """scale * table[tokens]: table [V, E] fp32 / bf16 / fp16 (row stride free), tokens int32 / int64 of any shape -> [*tokens.shape,
     E] of the table's type.  A token outside [0, V) gives a row of zeros."""
-    code, ld = _rows_of(table, "table")
+    code, ld, V, E = _rows_of(table, "table")
     N = _tokens_of(tokens, table.device)
-    V, E = table.shape
     out = torch.empty((*tokens.shape, E), dtype=table.dtype, device=table.device)
     if V == 0:
         return out.zero_()
@@ -1129,7 +1134,7 @@ def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.
         if not d_out.is_contiguous():
             raise ValueError("d_out: expected a contiguous tensor where tokens is not 1-d")
         d_out = d_out.view(tokens.numel(), E)
-    code, ld = _rows_of(d_out, "d_out")
+    code, ld, _, _ = _rows_of(d_out, "d_out")
     dev = d_out.device
     N = _tokens_of(tokens, dev)
     dtype = d_out.dtype if dtype is None else dtype
@@ -1137,7 +1142,7 @@ def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.
         raise ValueError(f"embedding_rows_grad: dtype must be {d_out.dtype} or float32, got {dtype}")
     if V < 0:
         raise ValueError("embedding_rows_grad: V < 0")
-    d_table = torch.empty((V, E), dtype=dtype, device=dev)
+    d_table = _new(V, E, dtype, dev)
     if N == 0 or V == 0 or E == 0:
         return d_table.zero_()
     nb = lib().phonlp_embedding_rows_grad_ws_bytes(N, E)
