@@ -416,11 +416,88 @@ def ner_loss(heads, params, enc, sentlens, tags, masks=None):
     return _loss_node(lambda e: heads.ner_backward(e, sentlens, tags, masks), enc, params)
 
 
+def _refuse_capture(name):
+    """A leaf that an eager graph still holds accumulates its gradient on the eager graph's stream; a captured backward that reaches
+    it ends the process inside the runtime, past any exception.  So the nodes refuse to be captured, forward and backward alike."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"phonlp_amd {name}: autograd nodes are not captured into a graph; capture the phonlp_amd.ops calls")
+
+
+class _EmbeddingRowsFn(torch.autograd.Function):
+    """out = scale * table[tokens]; the gradient of the table by sorted tokens (ops.embedding_rows / embedding_rows_grad)."""
+
+    @staticmethod
+    def forward(ctx, table, tokens, scale):
+        _refuse_capture("embedding_rows")
+        ctx.save_for_backward(tokens)
+        ctx.V, ctx.scale = table.shape[0], scale
+        return ops.embedding_rows(table, tokens, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        _refuse_capture("embedding_rows")
+        (tokens,) = ctx.saved_tensors
+        return ops.embedding_rows_grad(g.contiguous(), tokens, ctx.V, ctx.scale), None, None
+
+
+def embedding_rows(table, tokens, scale=1.0):
+    """Differentiable scale * table[tokens]: table [V, E] fp32 / bf16 / fp16, tokens int32 / int64 of any shape -> [*tokens.shape, E].
+    A token outside [0, V) gives a row of zeros and no gradient.  The gradient is summed in fp32 in an order that the tokens alone
+    fix (no float atomics), and rounded to the table's type once."""
+    return _EmbeddingRowsFn.apply(table, tokens.contiguous(), float(scale))
+
+
+class _LinearE4m3Fn(torch.autograd.Function):
+    """A dense layer on e4m3 images that keeps the images of its input and weight and, with a ReLU, one bit per output for its
+    backward: a byte where an fp32 layer keeps eight (ops.e4m3_rows / linear_e4m3 / linear_e4m3_backward)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, relu):
+        _refuse_capture("linear_e4m3")
+        K = x.shape[-1]
+        xi, wi = ops.e4m3_rows(x.reshape(x.shape[:-1].numel(), K).contiguous()), ops.e4m3_rows(weight.contiguous())
+        y, bits = ops.linear_e4m3(*xi, *wi, None if bias is None else bias.float().contiguous(), K, relu, x.dtype,
+                                  relu and any(ctx.needs_input_grad))
+        ctx.save_for_backward(*xi, *wi, bits)
+        ctx.K, ctx.shape = K, x.shape
+        ctx.types = weight.dtype, None if bias is None else bias.dtype
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        _refuse_capture("linear_e4m3")
+        *images, bits = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dX, dW, db = ops.linear_e4m3_backward(g.reshape(images[0].shape[0], images[2].shape[0]).contiguous(), bits, *images, ctx.K,
+                                              *need[:3])
+        return (None if dX is None else dX.view(ctx.shape), None if dW is None else dW.to(ctx.types[0]),
+                None if db is None else db.to(ctx.types[1]), None)
+
+
+def linear_e4m3(x, weight, bias=None, relu=False):
+    """Differentiable y = act(x @ weight.T + bias) with both operands in e4m3 (a power-of-two scale per row and block of 128 columns),
+    fp32 sums, y of x's type: x [..., K], weight [N, K], bias [N] in fp32 / bf16 / fp16.  What it keeps for the backward is the 8-bit
+    images and one bit per output of a ReLU; the quantisation counts as the identity.  Under torch.no_grad nothing is kept."""
+    return _LinearE4m3Fn.apply(x, weight, bias, bool(relu))
+
+
 def _encode_train(model, tokens, first_subword):
-    """Encoder + first-sub-word gather with autograd through both (ref jointmodel/model.py:112-116)."""
+    """Encoder + first-sub-word gather with autograd through both (ref jointmodel/model.py:112-116).  On the device the gather is
+    embedding_rows of the encoder's B * S rows; its backward sums by sorted rows.  An index outside the sentence is an error where the
+    indices are on the host; on the device its row is zeros without a gradient."""
     dev = _dev()
     enc_dev = next(model.phobert.parameters()).device
     emb = model.phobert(tokens.to(enc_dev))[2][-1]
+    if emb.is_cuda and emb.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        B, S, E = emb.shape
+        first = first_subword.long()
+        if not first.is_cuda and first.numel() and not 0 <= int(first.min()) <= int(first.max()) < S:
+            raise IndexError(f"first_subword: expected indices below {S}, got {int(first.min())} to {int(first.max())}")
+        first = first.to(enc_dev)
+        rows = torch.where((first >= 0) & (first < S), first + torch.arange(B, device=enc_dev)[:, None] * S, -1)
+        return embedding_rows(emb.reshape(B * S, E).contiguous(), rows).float().to(dev)
     idx = first_subword.to(enc_dev).long().unsqueeze(-1).expand(-1, -1, emb.shape[-1])
     return torch.gather(emb, 1, idx).float().to(dev)
 
@@ -454,15 +531,17 @@ def _update(self, batch_dep=None, batch_pos=None, batch_ner=None, lambda_pos=1.0
     (draw_masks) and handed to the kernels' callers as inputs; the encoder trains as it is (its own dropout included)."""
     args = self.model.args
     p_drop, p_word = float(args.get("dropout", 0.0)), float(args.get("word_dropout", 0.0))
+    e4m3 = getattr(self, "_amd_dense", "f32") == "e4m3"
     self.model.train()
     h = refresh_heads(self.model)
+    h.cfg["e4m3_train"] = e4m3
     dev = h.w.trans.device
     params = {k: p for k, p in self.model.named_parameters() if not k.startswith("phobert.")}
     if "dep_hid.weight" not in params:  # a model that keeps its heads outside the module tree (tests/stub_model.py)
         params = {k: v for k, v in _head_state(self.model).items() if v.requires_grad}
-    train = p_drop > 0.0 or p_word > 0.0
+    train = p_drop > 0.0 or p_word > 0.0 or e4m3  # the 8-bit layers are those of the training-mode pass
     if train and h.w.repl_dep is None:
-        raise ValueError("phonlp_amd update(): word dropout needs the training model's drop_replacement_* parameters")
+        raise ValueError("phonlp_amd update(): word dropout and dense='e4m3' need the training model's drop_replacement_* parameters")
 
     def masks(task, enc, lens):
         return draw_masks(h, task, enc.shape[0], enc.shape[1], lens, p_drop, p_word, dev) if train else None
@@ -482,14 +561,20 @@ def _update(self, batch_dep=None, batch_pos=None, batch_ner=None, lambda_pos=1.0
     return vals
 
 
-def patch_trainer(trainer, device=None, move_encoder=True, train_seam=False):
+def patch_trainer(trainer, device=None, move_encoder=True, train_seam=False, dense="f32"):
     """The evaluation-loop twin of patch(): rebinds `predict_dep`, `predict_pos` and `predict_ner` of a reference
     `JointTrainer` (models/jointmodel/trainer.py) so that the dev/test scoring loops of the training script run the
     heads and decoders on the MI355X, and adds `dev_loss` (the loss values of `update` on held-out batches).  `trainer.model` (jointmodel/model.py JointModel) keeps its encoder and its
     training-mode forward; only the eval-mode seams change.  The seams follow the live parameters: they re-pack the
     head weights (refresh_heads) when an optimizer step or load_state_dict changed them since the last call.
     `train_seam=True` also rebinds `update` (trainer.py:62-99): the three losses and their backward through the heads on
-    the HIP path as autograd nodes, the heads' dropout masks drawn per step and passed in."""
+    the HIP path as autograd nodes, the heads' dropout masks drawn per step and passed in.  `dense="e4m3"` (with train_seam)
+    runs that step's large dense layers (upos_hid, dep_hid, the scorers' first layers) on 8-bit images, forward and backward;
+    every other seam stays fp32."""
+    if dense not in ("f32", "e4m3"):
+        raise ValueError(f"patch_trainer: dense must be 'f32' or 'e4m3', got {dense!r}")
+    if dense == "e4m3" and not train_seam:
+        raise ValueError("patch_trainer: dense='e4m3' is the training seam's (train_seam=True)")
     dev = device or _dev()
     model = trainer.model
     if move_encoder:
@@ -499,6 +584,7 @@ def patch_trainer(trainer, device=None, move_encoder=True, train_seam=False):
     trainer.predict_pos = types.MethodType(_predict_pos, trainer)
     trainer.predict_ner = types.MethodType(_predict_ner, trainer)
     trainer.dev_loss = types.MethodType(_dev_loss, trainer)  # no counterpart by name: `update` minus dropout and backward
+    trainer._amd_dense = dense
     if train_seam:
         trainer.update = types.MethodType(_update, trainer)
     return trainer

@@ -229,6 +229,18 @@ class HeadWeights:
         return out.view(O, KPC // 32, 32, KP).permute(1, 0, 2, 3).contiguous().view(O * KPC, KP)
 
 
+def _dense(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor, relu: bool, e4m3: bool):
+    """One dense layer of a training step, x [M, K] fp32 -> (y [M, N], backward(dY) -> (dX, dW, db)).  e4m3: the product on the 8-bit
+    images of x and W, and the backward from the image of x and one bit per output in place of x and y."""
+    if not e4m3:
+        y = ops.linear(x, W, b, relu, None, 0)
+        return y, lambda dY: ops.linear_backward(x, W, y if relu else None, dY, relu)
+    K = x.shape[1]
+    xi, wi = ops.e4m3_rows(x), ops.e4m3_rows(W)
+    y, bits = ops.linear_e4m3(*xi, *wi, b, K, relu, torch.float32, relu)
+    return y, lambda dY: ops.linear_e4m3_backward(dY, bits, *xi, *wi, K)
+
+
 class TaskHeads:
     """POS + NER + dependency heads on the GPU.  All inputs/outputs are device tensors."""
 
@@ -250,6 +262,9 @@ class TaskHeads:
             # engine 2, sentences of up to 512 words: the arc scorers' stages A and B in one kernel, fed by the image the
             # W1/W2 layer writes (0: stage A as a GEMM of its own, stage B converting fp32 operands: the round-2 form)
             "arc_fused": env("PHONLP_ARC_FUSED", "1") == "1",
+            # the training step's large dense layers (upos_hid, dep_hid, the scorers' first layers) on e4m3 images
+            # (patch_trainer(dense="e4m3")); the decoders and every eval-mode pass stay as they are
+            "e4m3_train": False,
         }
         self._side = None
         # what the arc scorers' first layer gives a padded word (zero hidden row): relu of the layer's own bias
@@ -419,12 +434,12 @@ class TaskHeads:
         return torch.where(m.reshape(-1, 1), repl.reshape(1, -1).expand_as(x), x).contiguous()
 
     @staticmethod
-    def _soft_pos_train(w, x, emb, m_wd, m_drop):
+    def _soft_pos_train(w, x, emb, m_wd, m_drop, e4m3=False):
         """pos_forward(use_soft_pos=True) in .train() (ref jointmodel/model.py:125-137): word dropout on the encoder rows x [M,E]
         (rows m_wd -> drop_replacement_pos), ReLU(upos_hid), dropout mask m_drop [M,Hp] (kept entries 1/(1-p)), upos_clf,
         softmax, @ emb.  w: the HeadWeights.  -> (pos_emb [M,TE], upos logits, backward(d_pos_emb) -> (d_x, d_emb, {gradients}))."""
         xp = TaskHeads._word_drop(x, m_wd, w.repl_pos)
-        hid = ops.linear(xp, w.upos_hid_w, w.upos_hid_b, True, None, 0)
+        hid, hid_bw = _dense(xp, w.upos_hid_w, w.upos_hid_b, True, e4m3)
         hid_d = (hid * m_drop).contiguous()
         logits = ops.linear(hid_d, w.upos_clf_w, w.upos_clf_b, False, None, 0)
         P = ops.softmax_rows(logits.contiguous())
@@ -437,7 +452,7 @@ class TaskHeads:
             d_P, d_embT, _ = ops.linear_backward(P, emb.t().contiguous(), None, d_pos_emb.contiguous(), False, need_db=False)
             d_logits = ops.softmax_rows_backward(P, d_P)
             d_hid_d, dWc, dbc = ops.linear_backward(hid_d, w.upos_clf_w, None, d_logits, False)
-            d_xp, dWh, dbh = ops.linear_backward(xp, w.upos_hid_w, hid, (d_hid_d * m_drop).contiguous(), True)
+            d_xp, dWh, dbh = hid_bw((d_hid_d * m_drop).contiguous())
             keep = (~m_wd).reshape(-1, 1).to(d_xp.dtype)
             g = {"upos_hid.weight": dWh, "upos_hid.bias": dbh, "upos_clf.weight": dWc, "upos_clf.bias": dbc,
                  "drop_replacement_pos": (d_xp * (1.0 - keep)).sum(0)}
@@ -471,12 +486,14 @@ class TaskHeads:
         gh, gr = with_root(gold_head), with_root(gold_rel)
         live = (torch.arange(L, device=dev)[None, :] < lens[:, None]).reshape(M, 1)
         x = enc.reshape(M, E).contiguous()
-        pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_dep, bl(masks["wd_pos"]), f32(masks["drop_pos"]).reshape(M, -1))
+        pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_dep, bl(masks["wd_pos"]), f32(masks["drop_pos"]).reshape(M, -1),
+                                                       self.cfg["e4m3_train"])
         feat = torch.cat([x, pos_emb], 1).contiguous()
         m_wd = bl(masks["wd"])
         featd = TaskHeads._word_drop(feat, m_wd, w.repl_dep)
         # dep_hid; the padded rows of its output are the zeros of pad_packed_sequence (:182-183)
-        hidden = (ops.linear(featd, w.dep_hid_w, w.dep_hid_b, False, None, 0) * live).contiguous()
+        hidden, hidden_bw = _dense(featd, w.dep_hid_w, w.dep_hid_b, False, self.cfg["e4m3_train"])
+        hidden = (hidden * live).contiguous()
 
         def first_layer(name, W12, b12, row0):
             """A scorer's X1' | X2' [M, 2KP] from its two masked copies of `hidden`, plus what its backward needs."""
@@ -488,9 +505,14 @@ class TaskHeads:
                 Wk, bk = W12[row0 + k * KP:row0 + (k + 1) * KP].contiguous(), b12[row0 + k * KP:row0 + (k + 1) * KP].contiguous()
                 mk = torch.ones((M, KP), dtype=torch.float32, device=dev)  # the ones column (appended behind the dropout) stays
                 mk[:, :H] = f32(ms[k]).reshape(M, H)
-                y = (ops.linear(hin, Wk, bk, True, None, 0) * mk).contiguous()
+                if self.cfg["e4m3_train"]:
+                    y, layer_bw = _dense(hin, Wk, bk, True, True)
+                    y = (y * mk).contiguous()
+                else:  # the masked output carries the ReLU's mask: dropped entries get no gradient either way
+                    y = (ops.linear(hin, Wk, bk, True, None, 0) * mk).contiguous()
+                    layer_bw = lambda dY, hin=hin, Wk=Wk, y=y: ops.linear_backward(hin, Wk, y, dY, True)
                 out[:, k * KP:(k + 1) * KP] = y
-                saved.append((hin, Wk, mk, y, f32(mh[k]).reshape(M, D)))
+                saved.append((layer_bw, mk, f32(mh[k]).reshape(M, D)))
             return out, saved
 
         names = [nm for nm, on in zip(SCORERS, (True, w.linearization and n > 1, w.distance and n > 1)) if on]
@@ -519,9 +541,8 @@ class TaskHeads:
         def first_layer_backward(name, dXF_s, saved):
             nonlocal d_hidden
             for k, wn in enumerate(("W1", "W2")):
-                hin, Wk, mk, y, mhk = saved[k]
-                dY = (dXF_s[:, k * KP:(k + 1) * KP] * mk).contiguous()
-                d_hin, dW, db = ops.linear_backward(hin, Wk, y, dY, True)
+                layer_bw, mk, mhk = saved[k]
+                d_hin, dW, db = layer_bw((dXF_s[:, k * KP:(k + 1) * KP] * mk).contiguous())
                 grads[f"{name}.{wn}.weight"], grads[f"{name}.{wn}.bias"] = dW[:H], db[:H]
                 d_hidden = d_hidden + d_hin * mhk
 
@@ -537,7 +558,7 @@ class TaskHeads:
         grads["deprel.scorer.W_bilin.weight"] = unpack_bilinear(dWbtl, O)
         first_layer_backward("deprel", dXFl, saved_lab)
         d_live = (d_hidden * live).contiguous()
-        d_featd, dWd, dbd = ops.linear_backward(featd, w.dep_hid_w, None, d_live, False)
+        d_featd, dWd, dbd = hidden_bw(d_live)
         grads["dep_hid.weight"], grads["dep_hid.bias"] = dWd, dbd
         keep = (~m_wd).reshape(M, 1).to(torch.float32)
         grads["drop_replacement_dep"] = (d_featd * (1.0 - keep)).sum(0)
@@ -586,7 +607,8 @@ class TaskHeads:
             live = (torch.arange(L, device=dev)[None, :] < lens[:, None]).reshape(M, 1)
             x = enc.reshape(M, E).contiguous()
             pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_ner, bl(masks["wd_pos"]),
-                                                           torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1))
+                                                           torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1),
+                                                           self.cfg["e4m3_train"])
             m_wd = bl(masks["wd"])
             featd = TaskHeads._word_drop(torch.cat([x, pos_emb], 1).contiguous(), m_wd, w.repl_ner)
             logits2 = (ops.linear(featd, w.ner_w, w.ner_b, True, None, 0) * live).contiguous()
@@ -634,7 +656,7 @@ class TaskHeads:
             m_wd = torch.as_tensor(masks["wd_pos"]).to(device=dev, dtype=torch.bool).reshape(M)
             m_dp = torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1)
             xp = TaskHeads._word_drop(x, m_wd, w.repl_pos)
-            hid = ops.linear(xp, w.upos_hid_w, w.upos_hid_b, True, None, 0)
+            hid, hid_bw = _dense(xp, w.upos_hid_w, w.upos_hid_b, True, self.cfg["e4m3_train"])
             hid_d = (hid * m_dp).contiguous()
             logits = ops.linear(hid_d, w.upos_clf_w, w.upos_clf_b, False, None, 0).view(B, L, -1)
             gold = torch.as_tensor(gold_upos).to(device=dev, dtype=torch.int32).contiguous()
@@ -642,7 +664,7 @@ class TaskHeads:
             d_logits = ops.pos_loss_grad(logits, gold, lens, loss, ignore_index)
             U = logits.shape[2]
             d_hid_d, dWc, dbc = ops.linear_backward(hid_d, w.upos_clf_w, None, d_logits.reshape(M, U).contiguous(), False)
-            d_xp, dWh, dbh = ops.linear_backward(xp, w.upos_hid_w, hid, (d_hid_d * m_dp).contiguous(), True)
+            d_xp, dWh, dbh = hid_bw((d_hid_d * m_dp).contiguous())
             keep = (~m_wd).reshape(M, 1).to(torch.float32)
             return {"loss": loss, "d_enc": (d_xp * keep).view(B, L, E),
                     "grads": {"upos_hid.weight": dWh, "upos_hid.bias": dbh, "upos_clf.weight": dWc, "upos_clf.bias": dbc,

@@ -984,7 +984,7 @@ def _rows_of(t: Tensor, name: str):
         raise ValueError(f"{name}: expected 2 dimensions, got {len(shape)}")
     rows, cols = shape
     ld, step = t.stride()
-    if cols > 1 and step != 1 or rows > 1 and ld < cols:
+    if rows and (cols > 1 and step != 1 or rows > 1 and ld < cols):  # an empty tensor's strides say nothing
         raise ValueError(f"{name}: expected rows of unit column stride that do not overlap (pass .contiguous())")
     return code, ld if rows > 1 else cols, rows, cols
 

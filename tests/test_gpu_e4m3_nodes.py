@@ -1,0 +1,296 @@
+"""The 8-bit dense layer and the embedding lookup as autograd nodes (phonlp_amd.compat.linear_e4m3 / embedding_rows), run together as
+a model runs them, and the training seam with patch_trainer(dense="e4m3") -- against the definitions in 64 bits.
+
+Tolerances.  u32 = 2^-24, half an fp32 step; u = torch.finfo(t).eps / 2 of the result's type t.  A sum of n exact products in fp32 is
+off by at most 2 * n * u32 * sum|p| to first order: n additions in any order, each off by half a step where it rounds and a whole one
+where the matrix instruction cuts.  The products are exact: e4m3 values hold four bits, the pieces that a gradient is cut into eight,
+and a piece adds one term each (three for fp32).  A 16-bit result adds 7 * 2^-13 * sum|p|: the 8-bit pipe sums eight products at a time
+and cuts each 13 bits below the largest of them.  The last rounding to t adds u * |result|, or half a step of t's subnormals."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import e4m3_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    from phonlp_amd import _lib
+    _lib.lib()
+    return torch.device("cuda:0")
+
+
+def _round(t, want):
+    return torch.finfo(t).eps / 2 * np.maximum(np.abs(want), torch.finfo(t).smallest_normal)
+
+
+def _f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _within(got, want, bound, what):
+    err = np.abs(_f64(got) - want)
+    assert got.shape == want.shape, what
+    assert (err <= bound).all(), f"{what}: {float((err - bound).max()):.3e} past its bound"
+
+
+def _image_values(x):
+    return oracle.values(*oracle.image(x), x.shape[1])
+
+
+def _layer(xv, wv, b, relu, dtype):
+    """-> (exact result, bound on the kernel's)."""
+    y = oracle.linear(xv, wv, b, relu)
+    mag = np.abs(xv) @ np.abs(wv).T + np.abs(b)
+    n = 2 * xv.shape[1] + 2
+    cut = 0.0 if dtype == torch.float32 else 7 * 2.0 ** -13 * mag
+    return y, n * U32 * mag + cut + _round(dtype, y)
+
+
+def _check_backward(dy, bits, xv, wv, dX, dW, db, dtype, wtype, what):
+    """dy [M, N] 64-bit values of the incoming gradient, bits the mask that the forward kept."""
+    want = oracle.backward(dy, bits, xv, wv)
+    dz = np.abs(np.where(bits, dy, 0.0))
+    M, N = dz.shape
+    for got, w, mag, n, t in ((dX, want[0], dz @ np.abs(wv), 3 * N, dtype), (dW, want[1], dz.T @ np.abs(xv), 3 * M, wtype),
+                              (db, want[2], dz.sum(0), 3 * M, torch.float32)):
+        if got is not None:
+            _within(got, w, (2 * n + 2) * U32 * mag + _round(t, w), what)
+
+
+@pytest.mark.parametrize("lead", [(1,), (3, 7), (2, 5, 33)])
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_layer_node(dev, lead, relu, dtype):
+    from phonlp_amd import compat
+    g = torch.Generator().manual_seed(len(lead) * 10 + relu)
+    K, N = 131, 37
+    x = torch.randn(*lead, K, generator=g).to(dev, dtype).requires_grad_(True)
+    w = (torch.randn(N, K, generator=g) / K ** 0.5).to(dev, dtype).requires_grad_(True)
+    b = torch.randn(N, generator=g).to(dev).requires_grad_(True)
+    dy = torch.randn(*lead, N, generator=g).to(dev, dtype)
+    y = compat.linear_e4m3(x, w, b, relu)
+    assert y.dtype == dtype and y.shape == (*lead, N)
+    M = x.numel() // K
+    xv, wv = _image_values(_f64(x).reshape(M, K)), _image_values(_f64(w))
+    want, bound = _layer(xv, wv, _f64(b), relu, dtype)
+    _within(y.reshape(M, N), want, bound, "y")
+    y.backward(dy)
+    assert x.grad.dtype == x.dtype and w.grad.dtype == w.dtype and b.grad.dtype == b.dtype and x.grad.shape == x.shape
+    mask = (_f64(y).reshape(M, N) > 0) if relu else np.ones((M, N), bool)
+    _check_backward(_f64(dy).reshape(M, N), mask, xv, wv, x.grad.reshape(M, K), w.grad, b.grad, dtype, dtype, f"{lead} {dtype}")
+
+
+def test_layer_node_with_what_is_not_asked_for(dev):
+    """Frozen operands, no bias, a gradient that arrives as a view with strides, no_grad, an empty batch."""
+    from phonlp_amd import compat
+    g = torch.Generator().manual_seed(3)
+    x, w = torch.randn(6, 200, generator=g).to(dev), torch.randn(32, 200, generator=g).to(dev)
+    xv, wv = _image_values(_f64(x)), _image_values(_f64(w))
+    dy = torch.randn(32, 6, generator=g).to(dev).t()
+    w.requires_grad_(True)
+    y = compat.linear_e4m3(x, w, None, True)
+    y.backward(dy)
+    assert x.grad is None
+    _check_backward(_f64(dy), _f64(y) > 0, xv, wv, None, w.grad, None, torch.float32, torch.float32, "frozen x")
+    x.requires_grad_(True)
+    y = compat.linear_e4m3(x, w.detach(), None, False)
+    y.sum().backward()  # an expanded incoming gradient, strides of zero
+    _check_backward(np.ones((6, 32)), np.ones((6, 32), bool), xv, wv, x.grad, None, None, torch.float32, torch.float32, "frozen w")
+    with torch.no_grad():
+        assert not compat.linear_e4m3(x, w, None, True).requires_grad
+    empty = torch.empty(0, 200, device=dev, requires_grad=True)
+    w.grad = None
+    compat.linear_e4m3(empty, w, None, True).sum().backward()
+    assert empty.grad.shape == (0, 200) and not w.grad.any()
+    with pytest.raises(RuntimeError):  # the nodes have one derivative
+        y = compat.linear_e4m3(x, w, None, False)
+        (first,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        first.sum().backward()
+
+
+def test_layer_gradient_against_differences(dev):
+    """Integers up to 15 are exact in an image whose block's largest is 14 or 15, so the layer is the plain product there.  The loss is
+    quadratic in y and y linear in each leaf: a central difference over a step of one is the gradient itself, and every number on the
+    way is an integer or a half that its type holds (|y| < 2^13; gradients below 2^21), so the two are equal."""
+    from phonlp_amd import compat
+    g = torch.Generator().manual_seed(8)
+    M, K, N = 5, 140, 9
+    draw = lambda *s: torch.randint(-7, 8, s, generator=g).float()
+    x, w, b = draw(M, K), draw(N, K), draw(N)
+    x[:, ::128] = w[:, ::128] = 14.0
+    c = draw(M, N)
+
+    def loss(x, w, b):
+        y = compat.linear_e4m3(x.to(dev), w.to(dev), b.to(dev), False).double()
+        return (y * y * 0.5 + y * c.to(dev)).sum()
+
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    loss(*leaves).backward()
+    for i, (r, k) in ((0, (2, 5)), (0, (4, 139)), (1, (0, 3)), (1, (8, 130)), (2, (4, 0))):
+        sides = []
+        for step in (1.0, -1.0):
+            moved = [t.clone() for t in (x, w, b)]
+            if i == 2:
+                moved[i][r] += step
+            else:
+                moved[i][r, k] += step
+            sides.append(float(loss(*moved)))
+        got = float(leaves[i].grad[r] if i == 2 else leaves[i].grad[r, k])
+        assert (sides[0] - sides[1]) / 2 == got, (i, r, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,E,shape", [(11, 70, (4, 9)), (200, 32, (1,)), (3, 8, (2, 130)), (50, 16, (0, 4))])
+def test_lookup_node(dev, dtype, V, E, shape):
+    from phonlp_amd import compat
+    g = torch.Generator().manual_seed(V)
+    table = torch.randn(V, E, generator=g).to(dev, dtype).requires_grad_(True)
+    tokens = torch.randint(-1, V + 1, shape, generator=g).to(dev)
+    d = torch.randn(*shape, E, generator=g).to(dev, dtype)
+    out = compat.embedding_rows(table, tokens, 0.75)
+    t, tok, dv = _f64(table), tokens.cpu().numpy().reshape(-1), _f64(d).reshape(-1, E)
+    want = oracle.embedding(t, tok, 0.75)
+    assert out.shape == (*shape, E)
+    _within(out.reshape(-1, E), want, U32 * np.abs(want) + _round(dtype, want), "rows")
+    out.backward(d)
+    want = oracle.embedding_grad(dv, tok, V, 0.75)
+    mag = oracle.embedding_grad(np.abs(dv), tok, V, 0.75)
+    _within(table.grad, want, (tokens.numel() + 2) * U32 * mag + _round(dtype, want), "d_table")
+    again = table.detach().clone().requires_grad_(True)
+    compat.embedding_rows(again, tokens, 0.75).backward(d)
+    assert torch.equal(again.grad, table.grad)  # the order of the sums is the tokens'
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_run_of_them(dev, dtype):
+    """Lookup -> ReLU layer -> layer, and back to the table: each stage against the definitions on what the stage before gave it."""
+    from phonlp_amd import compat
+    g = torch.Generator().manual_seed(21)
+    V, E, H, O = 90, 136, 200, 40
+    leaf = lambda *s: (torch.randn(*s, generator=g) / s[-1] ** 0.5).to(dev, dtype).requires_grad_(True)
+    table, w1, w2 = leaf(V, E), leaf(H, E), leaf(O, H)
+    b1, b2 = torch.randn(H, generator=g).to(dev).requires_grad_(True), torch.randn(O, generator=g).to(dev).requires_grad_(True)
+    tokens = torch.randint(0, V, (5, 47), generator=g).to(dev)
+    d = torch.randn(5, 47, O, generator=g).to(dev, dtype)
+    x = compat.embedding_rows(table, tokens, 2.0)
+    h = compat.linear_e4m3(x, w1, b1, True)
+    y = compat.linear_e4m3(h, w2, b2, False)
+    for t in (x, h):
+        t.retain_grad()
+    y.backward(d)
+    M = tokens.numel()
+    flat = lambda t: _f64(t).reshape(M, -1)
+    xv, hv = _image_values(flat(x)), _image_values(flat(h))
+    w1v, w2v = _image_values(_f64(w1)), _image_values(_f64(w2))
+    for got, (want, bound) in ((h, _layer(xv, w1v, _f64(b1), True, dtype)), (y, _layer(hv, w2v, _f64(b2), False, dtype))):
+        _within(got.reshape(M, -1), want, bound, "layer")
+    _check_backward(flat(d), np.ones((M, O), bool), hv, w2v, h.grad.reshape(M, H), w2.grad, b2.grad, dtype, dtype, "second layer")
+    _check_backward(flat(h.grad), flat(h) > 0, xv, w1v, x.grad.reshape(M, E), w1.grad, b1.grad, dtype, dtype, "first layer")
+    tok, dv = tokens.cpu().numpy().reshape(-1), flat(x.grad)
+    want, mag = oracle.embedding_grad(dv, tok, V, 2.0), oracle.embedding_grad(np.abs(dv), tok, V, 2.0)
+    _within(table.grad, want, (M + 2) * U32 * mag + _round(dtype, want), "d_table")
+
+
+def _train_model(z):
+    from tests.stub_model import StubJointModel
+    model = StubJointModel(z)
+    model.args.update({"dropout": 0.0, "word_dropout": 0.0})
+    g = torch.Generator().manual_seed(4)
+    E, D = model._heads["upos_hid.weight"].shape[1], model._heads["dep_hid.weight"].shape[1]
+    model._heads.update({"drop_replacement_pos": torch.randn(E, generator=g) / E ** 0.5,
+                         "drop_replacement_ner": torch.randn(D, generator=g) / D ** 0.5,
+                         "drop_replacement_dep": torch.randn(D, generator=g) / D ** 0.5})
+    for m in model.phobert.modules():
+        if isinstance(m, torch.nn.Dropout):
+            m.p = 0.0
+    for v in model._heads.values():
+        if v.is_floating_point():
+            v.requires_grad_(True)
+    return model
+
+
+class _Trainer:
+    def __init__(self, model):
+        self.model, self.vocab, self.use_cuda = model, model.vocab, True
+
+
+def test_training_seam_on_8_bit_layers(golden, monkeypatch):
+    """patch_trainer(train_seam=True, dense="e4m3"): update() goes through the 8-bit layers in both directions (counted), every
+    parameter that the fp32 step reaches gets a finite gradient, and a trainer without the switch on the same model goes back to
+    fp32 with its results as they were."""
+    from phonlp_amd import ops
+    from phonlp_amd.compat import patch_trainer
+    z = golden("trainer_small.npz")
+    T = lambda k: torch.from_numpy(z[k])
+    batches = ((T("dep_tokens"), T("dep_first"), T("dep_mask"), T("loss_gold_head"), T("dep_gold_rel"), int(z["dep_nwords"]),
+                z["dep_oidx"].tolist(), z["dep_lens"].tolist()),
+               (T("tag_tokens"), T("tag_first"), T("gold_upos"), z["tag_oidx"].tolist(), z["tag_lens"].tolist()),
+               (T("tag_tokens"), T("tag_first"), T("tag_mask"), T("gold_ner"), z["tag_oidx"].tolist(), z["tag_lens"].tolist()))
+    calls = {"linear_e4m3": 0, "linear_e4m3_backward": 0}
+    for name in calls:
+        plain = getattr(ops, name)
+
+        def counted(*a, name=name, plain=plain, **k):
+            calls[name] += 1
+            return plain(*a, **k)
+
+        monkeypatch.setattr(ops, name, counted)
+    model = _train_model(z)
+    grads = lambda: {k: v.grad.clone() for k, v in model._heads.items() if v.is_floating_point() and v.grad is not None}
+
+    def step(**kw):
+        for v in list(model._heads.values()) + list(model.phobert.parameters()):
+            v.grad = None
+        got = patch_trainer(_Trainer(model), move_encoder=False, train_seam=True, **kw).update(*batches, 0.4, 0.2, 0.4)
+        return got, grads()
+
+    base, base_grads = step()
+    assert calls == {"linear_e4m3": 0, "linear_e4m3_backward": 0}
+    got, got_grads = step(dense="e4m3")
+    assert calls["linear_e4m3"] >= 6 and calls["linear_e4m3"] == calls["linear_e4m3_backward"]
+    assert np.isfinite(got).all() and set(base_grads) <= set(got_grads)
+    assert all(bool(torch.isfinite(v).all()) for v in got_grads.values())
+    count = dict(calls)
+    again, again_grads = step()
+    assert calls == count and again == base
+    for k, v in base_grads.items():
+        torch.testing.assert_close(again_grads[k], v, rtol=1e-5, atol=1e-6 * float(v.abs().max()))
+
+
+def test_encoder_rows_through_the_lookup(dev, golden):
+    """The first-sub-word rows of an encoder on the device: the values that torch.gather gives, bit for bit; the encoder's output gets
+    the sums of the rows' gradients, padded words (index 0 again and again) among them; an index past the sentence is refused."""
+    from phonlp_amd import compat
+    z = golden("trainer_small.npz")
+    model = _train_model(z)
+    model.phobert.to(dev)
+    model.train()
+    tokens, first = torch.from_numpy(z["dep_tokens"]), torch.from_numpy(z["dep_first"])
+    kept = []
+
+    def keep(module, args, out):
+        out[2][-1].retain_grad()
+        kept.append(out[2][-1])
+
+    hook = model.phobert.register_forward_hook(keep)
+    rows = compat._encode_train(model, tokens, first)
+    hook.remove()
+    (emb,) = kept
+    idx = first.to(dev)[..., None].expand(-1, -1, emb.shape[-1])
+    assert torch.equal(rows, torch.gather(emb, 1, idx))
+    d = torch.randn(rows.shape, generator=torch.Generator().manual_seed(2)).to(dev)
+    rows.backward(d)
+    want = torch.zeros(emb.shape, dtype=torch.float64, device=dev).scatter_add_(1, idx, d.double())
+    mag = torch.zeros(emb.shape, dtype=torch.float64, device=dev).scatter_add_(1, idx, d.double().abs())
+    _within(emb.grad, _f64(want), first.shape[1] * U32 * _f64(mag), "d_emb")
+    past = first.clone()
+    past[0, 0] = tokens.shape[1]
+    with pytest.raises(IndexError, match="first_subword"):
+        compat._encode_train(model, tokens, past)
+    beyond = compat._encode_train(model, tokens, past.to(dev))
+    assert not beyond[0, 0].any() and torch.equal(beyond[0, 1:], rows[0, 1:])
