@@ -294,3 +294,62 @@ def test_encoder_rows_through_the_lookup(dev, golden):
         compat._encode_train(model, tokens, past)
     beyond = compat._encode_train(model, tokens, past.to(dev))
     assert not beyond[0, 0].any() and torch.equal(beyond[0, 1:], rows[0, 1:])
+
+
+def _dense_on_image_values(x, W, b, relu, e4m3):
+    """heads._dense with the definitions in place of the kernels: plain products in 64 bits on the values that the images stand for."""
+    assert e4m3
+    xv, wv = (torch.from_numpy(_image_values(_f64(t))).to(x.device) for t in (x, W))
+    y = xv @ wv.t() + b.double()
+    y = y.relu() if relu else y
+
+    def backward(dY):
+        dz = dY.double() * (y > 0) if relu else dY.double()
+        return (dz @ wv).float(), (dz.t() @ xv).float(), dz.sum(0).float()
+
+    return y.float(), backward
+
+
+@pytest.mark.parametrize("task", ["parser", "ner", "pos"])
+def test_training_pass_on_8_bit_layers(dev, golden, monkeypatch, task):
+    """The losses with dropout masks on 8-bit layers against the same pass with _dense_on_image_values: the layers' order, masks and
+    which gradient goes where.  The two differ by fp32 rounding alone, but a value that lies within it of a border between two codes
+    moves by a code: a share of about 2^-16 of the values (2^-20 of a value against code steps of 2^-4), each by at most 2^-3 of
+    itself, which is 2^-11 of a layer's norm.  Three layers in a row and their backward: 2^-8 of each gradient's norm."""
+    from phonlp_amd import HeadWeights, TaskHeads, compat, heads as heads_module
+    z = golden("train_dropout_small.npz")
+    tag = {"parser": "dep", "ner": "ner", "pos": "pos"}[task]
+    order = ("unlabeled", "deprel", "linearization", "distance")
+    m = lambda k: torch.from_numpy(z[f"{tag}0_m_{k}"])
+    masks = {"wd_pos": m("wd_pos"), "drop_pos": m("drop_pos")}
+    if task == "parser":
+        mh, ms = m("hidden"), m("scorer")
+        masks.update({"wd": m("wd"), "hidden": {n: (mh[i, 0], mh[i, 1]) for i, n in enumerate(order)},
+                      "scorer": {n: (ms[i, 0], ms[i, 1]) for i, n in enumerate(order)}})
+    elif task == "ner":
+        masks["wd"] = m("wd")
+
+    def run():
+        params = {k[2:]: torch.from_numpy(z[k]).to(dev).requires_grad_(True) for k in z.files if k.startswith("p_") and z[k].ndim > 0}
+        heads = TaskHeads(HeadWeights.from_state_dict({k: v.detach() for k, v in params.items()}, dev))
+        heads.cfg["e4m3_train"] = True
+        enc = torch.from_numpy(z[f"{tag}0_enc"]).to(dev).requires_grad_(True)
+        lens = z[f"{tag}0_lens"].tolist()
+        if task == "parser":
+            loss = compat.parser_loss(heads, params, enc, lens, torch.from_numpy(z["dep0_head"]), torch.from_numpy(z["dep0_rel"]),
+                                      int(z["dep0_nwords"]), masks=masks)
+        elif task == "ner":
+            loss = compat.ner_loss(heads, params, enc, lens, torch.from_numpy(z["ner0_tags"]), masks=masks)
+        else:
+            loss = compat.pos_loss(heads, params, enc, lens, torch.from_numpy(z["pos0_upos"]), masks=masks)
+        loss.backward()
+        return loss.detach(), {k: v.grad for k, v in params.items() if v.grad is not None} | {"enc": enc.grad}
+
+    loss, grads = run()
+    monkeypatch.setattr(heads_module, "_dense", _dense_on_image_values)
+    want_loss, want = run()
+    assert abs(float(loss - want_loss)) <= 2.0 ** -10 * abs(float(want_loss))
+    assert grads.keys() == want.keys()
+    for k in want:
+        off = float((grads[k] - want[k]).double().norm())
+        assert off <= 2.0 ** -8 * float(want[k].double().norm()) + 1e-12, f"{k}: {off:.3e}"
