@@ -407,7 +407,7 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(E4m3Args a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sums[wave][i * 16 + g * 4 + r][j * 16 + l16] = acc[i][j][r];
     __syncthreads();
-    // 128 threads: eight columns of a row each; 512 threads: two, but a byte of bits stays with one thread
+    // 128 threads, eight columns of a row each: a byte of bits is one thread's
     if (threadIdx.x >= 128) return;
     const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8, m = m0 + r, waves = min(8, blocks);
     if (m >= a.M) return;
@@ -447,6 +447,19 @@ static int launch_tile(E4m3Args a, hipStream_t st) {
     return check_launch("linear_e4m3_kernel");
 }
 
+// The tile with the least estimated time.  A tile takes so much per block and so much at its ends (us, measured on products of 128 to
+// 4096 columns, 512 to 65536 rows): 256 x 256, a workgroup per compute unit, in whole rounds; 128 x 128, two workgroups per compute unit,
+// whose ends fall into each other's blocks.  16-bit results: 16384 x 8192 x 4096 475 against 572 us, 8192 x 2448 x 868 35.6 against
+// 28.2, 2011 x 13464 x 408 29.6 against 27.3; fp32: 810 against 970, 62.8 against 46.2, 50 against 42.
+template <class T>
+static bool large_tile(int M, int N, int Kp) {
+    constexpr bool f32 = sizeof(T) == 4;
+    const int blocks = Kp / 128;
+    const double large = (double)ceil_div(M, 256) * ceil_div(N, 256) / 256., small = (double)ceil_div(M, 128) * ceil_div(N, 128) / 512. + 0.25;
+    return (double)(long)(large + 0.999) * ((f32 ? 2.5 : 1.58) * blocks + (f32 ? 18. : 9.)) <
+           small * ((f32 ? 1.7 : 0.98) * blocks + (f32 ? 6.5 : 4.3));
+}
+
 }  // namespace phonlp
 
 using namespace phonlp;
@@ -465,12 +478,14 @@ extern "C" int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponent
     ProfScope ps("linear_e4m3", st);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        // tiles of 128 x 128 would leave most compute units without work
-        if ((long)ceil_div(M, 32) * ceil_div(N, 32) <= 1024 && M <= 32 * 65535) {
+        // Up to so many 32 x 32 the few-row form is the faster one; tiles of 128 x 128 would leave most compute units without work (fp32:
+        // 256 x 868 x 868 6.2 against 11.0 us, 256 x 2448 x 868, 616 of them, 10.8 against 11.3, 2048 x 400 x 768, 832, 11.9 against 10.6;
+        // 16-bit: 256 x 868 x 868 6.2 against 7.3, 128 x 2448 x 868, 308, 8.0 against 7.2)
+        if ((long)ceil_div(M, 32) * ceil_div(N, 32) <= (sizeof(T) == 4 ? 640 : 256)) {
             hipLaunchKernelGGL((linear_e4m3_few_kernel<T>), dim3(ceil_div(N, 32), ceil_div(M, 32)), dim3(512), 0, st, a);
             return check_launch("linear_e4m3_few_kernel");
         }
-        if ((long)ceil_div(M, 256) * ceil_div(N, 256) >= 256) return launch_tile<256, 256, T>(a, st);
+        if (large_tile<T>(M, N, a.Kp)) return launch_tile<256, 256, T>(a, st);
         return launch_tile<128, 128, T>(a, st);
     });
 }

@@ -312,3 +312,22 @@ def test_graph_and_streams(dev):
         assert all(torch.equal(a, b) for a, b in zip(eager, want[i]))
         for k, (_, _, _, out) in enumerate(graphs):
             assert all(torch.equal(a, b) for a, b in zip(out, want[(i + k) % 3]))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (8190, 4090, 130), (4090, 4090, 300), (8190, 4090, 2100), (7680, 4352, 1100)])
+def test_linear_large_products(dev, dtype, M, N, K):
+    """Products large enough for the large tile (one to seventeen blocks; one and two tiles of a workgroup, whole ones and edges): whole
+    numbers, so the sums are exact and the results their roundings."""
+    from phonlp_amd import ops
+    g = torch.Generator().manual_seed(K)
+    x, w, bias = (_whole(g, *s, 7).to(dev) for s in ((M, K), (N, K), (1, N)))
+    bias = bias[0].contiguous()
+    xi, wi = ops.e4m3_rows(x), ops.e4m3_rows(w)
+    want = (x.double() @ w.double().t() + bias.double()).relu()
+    y, bits = ops.linear_e4m3(*xi, *wi, bias, K, True, dtype, True)
+    assert torch.equal(y, want.to(dtype))
+    for rows in (slice(0, 300), slice(M - 300, M)):
+        assert np.array_equal(bits[rows].cpu().numpy(), O.pack_bits((want[rows] > 0).cpu().numpy()))
+    y, _ = ops.linear_e4m3(*xi, *wi, None, K, False, dtype)
+    assert torch.equal(y, (x.double() @ w.double().t()).to(dtype))
