@@ -5,6 +5,8 @@
 // number of sorted places and writes the runs of equal tokens that lie inside, runs that reach over a border leave fp32 shares
 // that a second launch adds in order.  No float atomics: the result does not depend on the launch, and a token that holds a large
 // share of all places is summed by as many waves as its places fill.  Both directions are bound by memory.
+#include <type_traits>
+
 #include "e4m3.h"
 
 namespace phonlp {
@@ -22,15 +24,16 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, lon
                                                              T *out) {
     constexpr int VEC = 16 / sizeof(T), ROWS = 16;
     typedef typename Vec<T, VEC>::type Vt;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = (blockIdx.y * 64 + lane) * VEC,
-              left = E - col;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
+              left = E - from, col = E < VEC ? from : min(from, E - VEC);  // at a row's end some columns twice, the same values
     const long n0 = (blockIdx.x * 4L + wave) * ROWS;
     if (n0 >= N) return;  // the whole wave
     const int rows = (int)min((long)ROWS, N - n0), held = token_key(tokens, n0 + min(lane, rows - 1), V);
     int key[ROWS];
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) key[u] = __builtin_amdgcn_readlane(held, u);
-    if (left >= VEC) {
+    if (E >= VEC) {
+        if (left <= 0) return;
         Vt v[ROWS];
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) v[u] = *reinterpret_cast<const Vt *>(table + (key[u] < V ? key[u] : 0) * ld + col);
@@ -41,7 +44,7 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, lon
             for (int i = 0; i < VEC; ++i) o[i] = key[u] < V ? (T)((float)v[u][i] * scale) : (T)0.f;
             if (u < rows) *reinterpret_cast<Vt *>(out + (n0 + u) * E + col) = o;
         }
-    } else if (left > 0) {  // the one lane at a row's end that has less than VEC columns
+    } else if (left > 0) {
 #pragma unroll
         for (int u = 0; u < ROWS; ++u)
             if (u < rows)
@@ -50,35 +53,39 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, lon
     }
 }
 
-// ---- sorting, few tokens: a token's place is the number of (token, n) pairs before its own.  N^2 comparisons of two instructions
-// each, in one launch (8192 tokens: 4 us; a radix pass is two launches of 3 to 5).  A workgroup places 32 tokens, eight threads a token
-// count an eighth of the others each.
+// ---- sorting, few tokens: a token's place is the number of (token, n) pairs before its own.  N^2 comparisons in one launch; a workgroup
+// places 32 tokens, 32 threads a token count a share of the others each.  A gradient of eight columns takes 17 us for 4096 tokens and 21
+// for 8192, against 25 and 24 by radix passes; for 12288 37 against 26.
+constexpr int kPlaceThreads = 1024;
 template <class I>
-__global__ __launch_bounds__(256) void embedding_place_kernel(const I *tokens, int N, int V, int *order, int *sorted) {
-    __shared__ __attribute__((aligned(16))) int keys[2048];
-    __shared__ int counts[8][32];
+__global__ __launch_bounds__(kPlaceThreads) void embedding_place_kernel(const I *tokens, int N, int V, int *order, int *sorted) {
+    constexpr int TILE = 4096, THREADS = kPlaceThreads, PARTS = THREADS / 32, EACH = TILE / THREADS;
+    __shared__ __attribute__((aligned(16))) int keys[TILE];
+    __shared__ int counts[PARTS][32];
     const int own = threadIdx.x & 31, part = threadIdx.x >> 5, n0 = blockIdx.x * 32, n = n0 + own;
     const int key = n < N ? token_key(tokens, n, V) : 0;
     int count = 0;
-    for (int base = 0; base < N; base += 2048) {
+    for (int base = 0; base < N; base += TILE) {
         __syncthreads();
-        for (int i = threadIdx.x; i < min(2048, N - base + 4); i += 256)
-            if (i < 2048) keys[i] = base + i < N ? token_key(tokens, base + i, V) : 0x7FFFFFFF;
-        __syncthreads();
-        const int lo = part * 256;
-        if (base + lo >= N) continue;
-        // up to 256 tokens of this thread: those before this workgroup's 32, those 32 (all in one thread's share, or none), those behind;
-        // equal ones count if they stand before n
-        const int mine = min((N - base - lo + 3) & ~3, 256), split = min(max(n0 - base - lo, 0), mine),
-                  split32 = min(max(n0 + 32 - base - lo, 0), mine);
-        for (int i = 0; i < split; i += 4) {
-            const int4 k = *reinterpret_cast<const int4 *>(keys + lo + i);
-            count += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+        I t[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) t[i] = tokens[min(base + i * THREADS + (int)threadIdx.x, N - 1)];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = i * THREADS + threadIdx.x;
+            keys[at] = base + at >= N ? 0x7FFFFFFF : t[i] >= 0 && t[i] < (I)V ? (int)t[i] : V;
         }
-        for (int i = split; i < split32; ++i) count += keys[lo + i] < key + (base + lo + i < n ? 1 : 0);
-        for (int i = split32; i < mine; i += 4) {
-            const int4 k = *reinterpret_cast<const int4 *>(keys + lo + i);
-            count += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
+        __syncthreads();
+        // this thread's share of them, 32 at a time: equal ones count if they stand before n
+#pragma unroll 1
+        for (int i = part * (TILE / PARTS); i < (part + 1) * (TILE / PARTS) && base + i < N; i += 32) {
+            const int first = n0 - base - i, bound = key + (first > 0);  // first = 0: this workgroup's own 32
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const int4 k = *reinterpret_cast<const int4 *>(keys + i + j);
+                if (first) count += (k.x < bound) + (k.y < bound) + (k.z < bound) + (k.w < bound);
+                else count += (k.x < key + (j < own)) + (k.y < key + (j + 1 < own)) + (k.z < key + (j + 2 < own)) + (k.w < key + (j + 3 < own));
+            }
         }
     }
     counts[part][own] = count;
@@ -86,7 +93,7 @@ __global__ __launch_bounds__(256) void embedding_place_kernel(const I *tokens, i
     if (part == 0 && n < N) {
         int place = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) place += counts[i][own];
+        for (int i = 0; i < PARTS; ++i) place += counts[i][own];
         order[place] = n;
         sorted[place] = key;
     }
@@ -105,7 +112,14 @@ __global__ __launch_bounds__(256) void embedding_count_kernel(const I *tokens, c
     bins[threadIdx.x] = 0;
     __syncthreads();
     const long base = (long)blockIdx.x * tile;
-    for (int i = threadIdx.x; i < tile && base + i < N; i += 256) atomicAdd(&bins[sort_key(tokens, keys, base + i, V) >> shift & 255], 1);
+    for (int i = threadIdx.x; i < tile && base + i < N; i += 1024) {  // four loads in flight
+        int key[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) key[u] = sort_key(tokens, keys, min(base + i + u * 256, N - 1L), V);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (base + i + u * 256 < N) atomicAdd(&bins[key[u] >> shift & 255], 1);
+    }
     __syncthreads();
     counts[blockIdx.x * 256 + threadIdx.x] = bins[threadIdx.x];
 }
@@ -120,9 +134,21 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(const I *tokens,
 #pragma unroll
     for (int w = 0; w < 4; ++w) at[w][threadIdx.x] = 0;
     __syncthreads();
-    for (int r = 0; r < tile / 4; r += 64) {
-        const long n = base + r + lane;
-        if (n < N) atomicAdd(&at[wave][sort_key(tokens, keys, n, V) >> shift & 255], 1);
+    // four of the wave's pairs per lane at a time: those of the tile's first (and most often only) 256 stay in registers
+    int key[4], from[4];
+    auto read = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const long n = min(base + r + u * 64 + lane, N - 1L);
+            key[u] = sort_key(tokens, keys, n, V);
+            from[u] = index ? index[n] : (int)n;
+        }
+    };
+    for (int r = tile / 4 - 256; r >= 0; r -= 256) {
+        read(r);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (base + r + u * 64 + lane < N) atomicAdd(&at[wave][key[u] >> shift & 255], 1);
     }
     // this thread's digit: the pairs of smaller digits, and those of its own in the tiles before
     int total = 0, before = 0;
@@ -150,27 +176,30 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(const I *tokens,
         place += c;
     }
     __syncthreads();
-    for (int r = 0; r < tile / 4; r += 64) {
-        const long n = base + r + lane;
-        const bool in = n < N;
-        const int key = in ? sort_key(tokens, keys, n, V) : 0, digit = key >> shift & 255;
-        // the lanes that hold a pair of the same digit
-        unsigned long long same = __ballot(in);
+    for (int r = 0; r < tile / 4; r += 256) {
+        if (r) read(r);
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
-            const unsigned long long set = __ballot(digit >> b & 1);
-            same &= digit >> b & 1 ? set : ~set;
+        for (int u = 0; u < 4; ++u) {
+            const bool in = base + r + u * 64 + lane < N;
+            const int digit = key[u] >> shift & 255;
+            // the lanes that hold a pair of the same digit
+            unsigned long long same = __ballot(in);
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                const unsigned long long set = __ballot(digit >> b & 1);
+                same &= digit >> b & 1 ? set : ~set;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            int first = 0;
+            if (in) first = at[wave][digit];
+            __builtin_amdgcn_wave_barrier();
+            if (in) {
+                keys_out[first + rank] = key[u];
+                index_out[first + rank] = from[u];
+                if (rank == 0) at[wave][digit] = first + __popcll(same);
+            }
+            __builtin_amdgcn_wave_barrier();
         }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        int first = 0;
-        if (in) first = at[wave][digit];
-        __builtin_amdgcn_wave_barrier();
-        if (in) {
-            keys_out[first + rank] = key;
-            index_out[first + rank] = index ? index[n] : (int)n;
-            if (rank == 0) at[wave][digit] = first + __popcll(same);
-        }
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -185,27 +214,40 @@ __device__ __forceinline__ int lower_bound(const int *sorted, int lo, int hi, in
     return lo;
 }
 
-template <class T, int VEC>
-__device__ __forceinline__ void load_row(const T *p, int left, float (&v)[VEC]) {
-    typedef typename Vec<T, VEC>::type Vt;
-    if (left >= VEC) {
-        const Vt t = *reinterpret_cast<const Vt *>(p);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = (float)t[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+// The same by a whole wave, for a key that all its lanes have: 64 places a step.
+__device__ __forceinline__ int lower_bound_wave(const int *sorted, int n, int key, int lane) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int step = ceil_div(hi - lo, 64), at = lo + (lane + 1) * step - 1;
+        const int less = __popcll(__ballot(at < hi && sorted[min(at, hi - 1)] < key));
+        hi = min(hi, lo + (less + 1) * step - 1);
+        lo += less * step;
     }
+    return lo;
 }
-template <class TO, int VEC>
+
+// A lane's VEC columns of a row, from `col`; `left` of them are there.  WHOLE: E >= VEC, and a lane that would reach behind the row takes
+// its last VEC columns, some of them with its neighbour, which then both hold the same sums, and a lane behind it reads without need.
+// (A branch for every column of every row takes longer than the loads: 512 rows on one wave, eight columns of bf16 a lane, 247 us
+// against 121.)
+template <bool WHOLE, class T, int VEC>
+__device__ __forceinline__ typename Vec<T, VEC>::type load_raw(const T *row, int col, int left) {
+    typedef typename Vec<T, VEC>::type Vt;
+    if (WHOLE || left >= VEC) return *reinterpret_cast<const Vt *>(row + col);
+    Vt v;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = i < left ? row[col + i] : (T)0.f;
+    return v;
+}
+template <bool WHOLE, class TO, int VEC>
 __device__ __forceinline__ void store_row(TO *p, int left, const float (&v)[VEC], float scale) {
     typedef typename Vec<TO, VEC>::type Vt;
-    if (left >= VEC) {
+    if (WHOLE ? left > 0 : left >= VEC) {
         Vt t;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) t[i] = (TO)(v[i] * scale);
         *reinterpret_cast<Vt *>(p) = t;
-    } else {
+    } else if (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
             if (i < left) p[i] = (TO)(v[i] * scale);
@@ -223,7 +265,8 @@ struct SumArgs {
 };
 
 // blockIdx.y: a slab of 64 * VEC columns.  blockIdx.x < sum_blocks: a wave per chunk of R sorted places, sixteen rows in flight; behind
-// them (first slab only): a wave per 16 rows of the table, which writes zeros where no token points.
+// them (first slab only): a wave per 16 rows of the table, which writes zeros where no token points (64 tokens, 64000 x 768
+// bf16: 22.3 us with a search per row, 21.2 with one per 16).
 template <class T, class TO>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
     constexpr int VEC = 16 / sizeof(T), UNROLL = 16;
@@ -232,59 +275,65 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
     TO *table = (TO *)a.d_table;
     if ((int)blockIdx.x >= a.sum_blocks) {
         if (blockIdx.y) return;
-        const long row0 = ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 16, row = row0 + lane;
-        bool empty = false;
-        if (lane < 16 && row < a.V) {
-            const int at = lower_bound(a.sorted, 0, a.N, (int)row);
-            empty = at == a.N || a.sorted[at] != (int)row;
+        const long row0 = ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 16;
+        if (row0 >= a.V) return;
+        unsigned long long rows = (1ull << min(a.V - row0, 16L)) - 1;  // those that no token points at
+        const int from = lower_bound_wave(a.sorted, a.N, (int)row0, lane);
+        const int key = from + lane < a.N ? a.sorted[from + lane] : 0x7FFFFFFF;
+        if (__builtin_amdgcn_readlane(key, 63) >= row0 + 16) {  // the next 64 places hold all of their tokens
+#pragma unroll
+            for (int r = 0; r < 16; ++r) rows &= ~((unsigned long long)(__ballot(key == row0 + r) != 0) << r);
+        } else {
+            bool there = false;
+            if (lane < 16) {
+                const int at = lower_bound(a.sorted, from, a.N, (int)row0 + lane);
+                there = at < a.N && a.sorted[at] == row0 + lane;
+            }
+            rows &= ~__ballot(there);
         }
-        unsigned long long rows = __ballot(empty);
         constexpr int VO = 16 / sizeof(TO);
         const float zero[VO] = {};
         while (rows) {
             const int r = __ffsll(rows) - 1;
             rows &= rows - 1;
-            for (int c = lane * VO; c < a.E; c += 64 * VO) store_row<TO, VO>(table + (row0 + r) * a.E + c, a.E - c, zero, 0.f);
+            for (int c = lane * VO; c < a.E; c += 64 * VO) store_row<false, TO, VO>(table + (row0 + r) * a.E + c, a.E - c, zero, 0.f);
         }
         return;
     }
-    const int chunk = blockIdx.x * 4 + wave, col = (blockIdx.y * 64 + lane) * VEC, left = a.E - col;
+    const int chunk = blockIdx.x * 4 + wave, from = (blockIdx.y * 64 + lane) * VEC, left = a.E - from, col = a.E < VEC ? from : min(from, a.E - VEC);
     if (chunk >= a.chunks) return;
     const int first = chunk * a.R, last = min(first + a.R, a.N);
-    const T *d = (const T *)a.d_out + col;
-    bool head = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
-    float s[VEC] = {};
-    for (int p = first; p < last; p += UNROLL) {
-        // lane u holds place p + u
-        const int at = p + lane, row = a.order[min(at, last - 1)], key = at < a.N ? a.sorted[at] : -1;
-        Vt v[UNROLL];
+    const T *d = (const T *)a.d_out;
+    auto sum = [&](auto w) {
+        constexpr bool WHOLE = decltype(w)::value;
+        bool head = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
+        float s[VEC] = {};
+        for (int p = first; p < last; p += UNROLL) {
+            // lane u holds place p + u
+            const int at = p + lane, row = a.order[min(at, last - 1)], key = at < a.N ? a.sorted[at] : -1;
+            Vt v[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const T *q = d + (long)__builtin_amdgcn_readlane(row, u) * a.ld;
-            if (left >= VEC) {
-                v[u] = *reinterpret_cast<const Vt *>(q);
-            } else {
+            for (int u = 0; u < UNROLL; ++u) v[u] = load_raw<WHOLE, T, VEC>(d + (long)__builtin_amdgcn_readlane(row, u) * a.ld, col, left);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[u][i] = i < left ? q[i] : (T)0.f;
+            for (int u = 0; u < UNROLL; ++u) {
+                if (p + u >= last) break;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[i] += (float)v[u][i];
+                const int k = __builtin_amdgcn_readlane(key, u);
+                const bool ends = __builtin_amdgcn_readlane(key, u + 1) != k;
+                if (!ends && p + u + 1 < last) continue;
+                if (k < a.V) {
+                    if (ends && !head) store_row<WHOLE, TO, VEC>(table + (long)k * a.E + col, left, s, a.scale);
+                    else store_row<WHOLE, float, VEC>(a.shares + ((long)chunk * 2 + (head ? 0 : 1)) * a.E + col, left, s, 1.f);
+                }
+                head = false;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[i] = 0.f;
             }
         }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            if (p + u >= last) break;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) s[i] += (float)v[u][i];
-            const int k = __builtin_amdgcn_readlane(key, u);
-            const bool ends = __builtin_amdgcn_readlane(key, u + 1) != k;
-            if (!ends && p + u + 1 < last) continue;
-            if (left > 0 && k < a.V) {
-                if (ends && !head) store_row<TO, VEC>(table + (long)k * a.E + col, left, s, a.scale);
-                else store_row<float, VEC>(a.shares + ((long)chunk * 2 + (head ? 0 : 1)) * a.E + col, left, s, 1.f);
-            }
-            head = false;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) s[i] = 0.f;
-        }
-    }
+    };
+    if (a.E >= VEC) sum(std::true_type{});
+    else sum(std::false_type{});
 }
 
 // Runs that go on behind the chunk they begin in: their shares, in order.  A workgroup looks at eight chunks, a chunk per lane; runs of
@@ -293,8 +342,8 @@ template <class T, class TO>
 __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
     constexpr int VEC = 16 / sizeof(T), UNROLL = 16 / (VEC / 4), FEW = 16;
     __shared__ float sums[8][64 * VEC];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = (blockIdx.y * 64 + lane) * VEC,
-              left = a.E - col, mine = blockIdx.x * 8 + lane;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
+              left = a.E - from, col = a.E < VEC ? from : min(from, a.E - VEC), mine = blockIdx.x * 8 + lane;
     auto reaches = [&](int chunk, int k) {  // the first place of `chunk` still holds k
         const long p = (long)chunk * a.R;
         return (p < a.N) & (a.sorted[min(p, (long)a.N - 1)] == k);
@@ -309,13 +358,13 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
             for (int i = 2; i <= FEW; ++i) count += reaches(mine + i, k);
         }
     }
-    auto add = [&](int chunk, int lo, int hi, float (&s)[VEC]) {  // shares lo .. hi - 1: the chunk's last run, then the next chunks' first
+    auto add_as = [&](auto w, int chunk, int lo, int hi, float (&s)[VEC]) {
         for (int c = lo; c < hi; c += UNROLL) {
-            float v[UNROLL][VEC];
+            typename Vec<float, VEC>::type v[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int k = min(c + u, hi - 1);
-                load_row<float, VEC>(a.shares + ((long)(chunk + k) * 2 + (k ? 0 : 1)) * a.E + col, left, v[u]);
+                v[u] = load_raw<decltype(w)::value, float, VEC>(a.shares + ((long)(chunk + k) * 2 + (k ? 0 : 1)) * a.E, col, left);
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u)
@@ -323,6 +372,15 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
                 for (int i = 0; i < VEC; ++i)
                     if (c + u < hi) s[i] += v[u][i];
         }
+    };
+    auto add = [&](int chunk, int lo, int hi, float (&s)[VEC]) {  // shares lo .. hi - 1: the chunk's last run, then the next chunks' first
+        if (a.E >= VEC) add_as(std::true_type{}, chunk, lo, hi, s);
+        else add_as(std::false_type{}, chunk, lo, hi, s);
+    };
+    auto store = [&](int k, const float (&s)[VEC]) {
+        TO *p = (TO *)a.d_table + (long)k * a.E + col;
+        if (a.E >= VEC) store_row<true, TO, VEC>(p, left, s, a.scale);
+        else store_row<false, TO, VEC>(p, left, s, a.scale);
     };
     int turn = 0;
     for (unsigned long long runs = __ballot(key < a.V); runs; runs &= runs - 1) {
@@ -336,7 +394,7 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
         if (n <= FEW + 1) {
             if ((turn++ & 7) == wave && left > 0) {
                 add(chunk, 0, n, s);
-                store_row<TO, VEC>((TO *)a.d_table + (long)k * a.E + col, left, s, a.scale);
+                store(k, s);
             }
             continue;
         }
@@ -350,13 +408,13 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
             for (int w = 1; w < 8; ++w)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) s[i] += sums[w][i * 64 + lane];
-            store_row<TO, VEC>((TO *)a.d_table + (long)k * a.E + col, left, s, a.scale);
+            store(k, s);
         }
         __syncthreads();
     }
 }
 
-constexpr int kPlaceMost = 8192;
+constexpr int kPlaceMost = 8192;  // tokens sorted by counting (above)
 struct EmbeddingPlan {
     int R, chunks, tile, tiles;  // places of one wave; pairs of a sorting tile
     size_t pairs, shares, counts, total;
@@ -380,7 +438,7 @@ static int sort_tokens(const I *tokens, int N, int V, const EmbeddingPlan &pl, c
     ProfScope ps("embedding_sort", st);
     int *k[2] = {(int *)ws, (int *)(ws + pl.pairs)};
     if (N <= kPlaceMost) {
-        hipLaunchKernelGGL((embedding_place_kernel<I>), dim3(ceil_div(N, 32)), dim3(256), 0, st, tokens, N, V, k[0], k[1]);
+        hipLaunchKernelGGL((embedding_place_kernel<I>), dim3(ceil_div(N, 32)), dim3(kPlaceThreads), 0, st, tokens, N, V, k[0], k[1]);
         *order = k[0];
         *sorted = k[1];
         return check_launch("embedding_place_kernel");
