@@ -142,3 +142,25 @@ def test_graph(dev):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
             assert all(torch.equal(a, b) for a, b in zip(eager, want[(i + 1) % 3]))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("N", [31, 32, 33, 4095, 4097, 8191])
+@pytest.mark.parametrize("E", [7, 13, 520])
+def test_rows_of_a_wider_tensor(dev, dtype, N, E):
+    """Rows inside a wider tensor of NaN: row ends of every kind (less than one vector; a last vector that overlaps its neighbour; over
+    two slabs), counts on both sides of the sorts' steps.  Whole numbers: exact."""
+    from phonlp_amd import ops
+    g = torch.Generator().manual_seed(N + E)
+    V = 50
+    tokens = _tokens(g, N, V, "outside")
+    wide = torch.full((max(N, V), E + 11), float("nan"), dtype=dtype, device=dev)
+    table, d_out = torch.randint(-100, 101, (V, E), generator=g).to(dtype), torch.randint(-3, 4, (N, E), generator=g).to(dtype)
+    part = wide[:V, 5:5 + E]
+    part.copy_(table)
+    out = ops.embedding_rows(part, tokens.to(dev), 1.0)
+    assert np.array_equal(_np(out), O.embedding(_np(table), tokens.numpy(), 1.0))
+    part = wide[:N, 5:5 + E]
+    part.copy_(d_out)
+    grad = ops.embedding_rows_grad(part, tokens.to(dev), V, 1.0, torch.float32)
+    assert torch.equal(grad.cpu(), torch.from_numpy(O.embedding_grad(_np(d_out), tokens.numpy(), V, 1.0)).float())
