@@ -1,19 +1,19 @@
 // Matrix <-> e4m3 image (e4m3.h): the operand form of phonlp_linear_e4m3 and, at a quarter of fp32's bytes, the checkpoint of a
 // layer's input that phonlp_linear_e4m3_backward reads.  One pass, memory-bound: a block of 128 columns is held by 32 (fp32) or 16
 // (16-bit types) neighbouring lanes with one 16-byte load each, its largest magnitude is found with lane permutations, and the
-// codes leave as one 4- or 8-byte store per lane.
+// codes leave as one 4- or 8-byte store per lane.  32768 x 868 fp32: 29 us to the image, 26 back, 5 TB/s, the rate of a copy.
+#include <type_traits>
+
 #include "e4m3.h"
 
 namespace phonlp {
 
-__device__ __forceinline__ int max_xor_dpp(int v, int other) { return v > other ? v : other; }
-
 // Largest value over the aligned group of 16 lanes that a lane belongs to (quads, then halves, then the row mirrored).
 __device__ __forceinline__ int group16_max(int v) {
-    v = max_xor_dpp(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
-    v = max_xor_dpp(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
-    v = max_xor_dpp(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
-    v = max_xor_dpp(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
     return v;
 }
 
@@ -88,8 +88,10 @@ __global__ __launch_bounds__(256) void e4m3_rows_kernel(const T *x, long ldx, in
 }
 
 // Values of an image, in T.  16-bit types saturate: an e4m3 code may stand for a little more than the block's largest entry was
-// (fp16: 65504 becomes 256 * 2^8).  fp32's largest is kept by the quantiser itself.
-template <class T, int VEC>
+// (fp16: 65504 becomes 256 * 2^8).  fp32's largest is kept by the quantiser itself.  RAGGED: K is no multiple of VEC, and a row's last
+// vector begins VEC columns before its end, some of them its neighbour's as well, perhaps in two blocks (32768 x 867 bf16: 17 us, one
+// column a thread 57).
+template <class T, int VEC, bool RAGGED>
 __global__ __launch_bounds__(256) void e4m3_values_kernel(const uint8_t *codes, const uint8_t *exponents, int M, int K, int Kp, int KB4,
                                                           T *out) {
     typedef typename Vec<T, VEC>::type V;
@@ -98,26 +100,32 @@ __global__ __launch_bounds__(256) void e4m3_values_kernel(const uint8_t *codes, 
     constexpr int UNROLL = 4;
     for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < total; g += step * UNROLL) {
         uint8_t c[UNROLL][VEC];
-        uint8_t e[UNROLL];
+        uint8_t e[UNROLL], e2[UNROLL];
+        int border[UNROLL];  // from this one on the vector's columns are the next block's
         long at[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const long it = g + u * step;
             if (it >= total) continue;
             const long row = total < (1L << 31) ? (long)((unsigned)it / (unsigned)per_row) : it / per_row;
-            const int k = (int)(it - row * per_row) * VEC;
+            int k = (int)(it - row * per_row) * VEC;
+            if (RAGGED) k = min(k, K - VEC);
             at[u] = row * K + k;
-            __builtin_memcpy(c[u], codes + row * Kp + k, VEC);  // VEC divides 128: inside the padded row
+            __builtin_memcpy(c[u], codes + row * Kp + k, VEC);
             e[u] = exponents[row * KB4 + (k >> 7)];
+            if (RAGGED) {
+                e2[u] = exponents[row * KB4 + ((k + VEC - 1) >> 7)];
+                border[u] = 128 - (k & 127);
+            }
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             if (g + u * step >= total) continue;
-            const float scale = exp2_biased(e[u] < 1 ? 1 : e[u]);
+            const float scale = exp2_biased(e[u] < 1 ? 1 : e[u]), scale2 = RAGGED ? exp2_biased(e2[u] < 1 ? 1 : e2[u]) : scale;
             V o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                float v = __builtin_amdgcn_cvt_f32_fp8(c[u][i], 0) * scale;
+                float v = __builtin_amdgcn_cvt_f32_fp8(c[u][i], 0) * (RAGGED && i >= border[u] ? scale2 : scale);
                 if (sizeof(T) == 2) {
                     const float top = __is_same(T, _Float16) ? 65504.f : 3.3895313892515355e38f;
                     v = v > top ? top : v < -top ? -top : v;  // keeps NaN
@@ -168,16 +176,14 @@ extern "C" int phonlp_e4m3_values(const void *codes, const uint8_t *exponents, i
         using T = decltype(t);
         constexpr int VEC = 16 / sizeof(T);
         const uint8_t *c = (const uint8_t *)codes;
-        // a row of K values is cut into vectors only if they end with the row
-        if (K % VEC == 0)
-            hipLaunchKernelGGL((e4m3_values_kernel<T, VEC>), dim3(rows_grid((long)rows * (K / VEC), 256)), dim3(256), 0, st, c, exponents,
-                               rows, K, kp8_of(K), kb4_of(K), (T *)out);
-        else if (K % (VEC / 2) == 0)
-            hipLaunchKernelGGL((e4m3_values_kernel<T, VEC / 2>), dim3(rows_grid((long)rows * (K / (VEC / 2)), 256)), dim3(256), 0, st, c,
-                               exponents, rows, K, kp8_of(K), kb4_of(K), (T *)out);
-        else
-            hipLaunchKernelGGL((e4m3_values_kernel<T, 1>), dim3(rows_grid((long)rows * K, 256)), dim3(256), 0, st, c, exponents, rows, K,
-                               kp8_of(K), kb4_of(K), (T *)out);
+        auto launch = [&](auto vec, auto ragged) {
+            constexpr int V = decltype(vec)::value;
+            hipLaunchKernelGGL((e4m3_values_kernel<T, V, decltype(ragged)::value>), dim3(rows_grid((long)rows * ((K + V - 1) / V), 256)),
+                               dim3(256), 0, st, c, exponents, rows, K, kp8_of(K), kb4_of(K), (T *)out);
+        };
+        if (K % VEC == 0) launch(std::integral_constant<int, VEC>{}, std::false_type{});
+        else if (K > VEC) launch(std::integral_constant<int, VEC>{}, std::true_type{});
+        else launch(std::integral_constant<int, 1>{}, std::false_type{});
         return check_launch("e4m3_values_kernel");
     });
 }
