@@ -331,3 +331,28 @@ def test_linear_large_products(dev, dtype, M, N, K):
         assert np.array_equal(bits[rows].cpu().numpy(), O.pack_bits((want[rows] > 0).cpu().numpy()))
     y, _ = ops.linear_e4m3(*xi, *wi, None, K, False, dtype)
     assert torch.equal(y, (x.double() @ w.double().t()).to(dtype))
+
+
+def test_products_past_32_bit_offsets(dev):
+    """More than 2^31 outputs: the last rows of Y, its bits and dX, and dW and db over all of them (entries of -1, 0 and 1: every sum is
+    exact)."""
+    from phonlp_amd import ops
+    M, N, K = 1_060_003, 2100, 131
+    assert M * N > 2 ** 31
+    g = torch.Generator(device=dev).manual_seed(3)
+    draw = lambda *s: torch.randint(-1, 2, s, generator=g, device=dev, dtype=torch.int8)
+    x, w, dy = draw(M, K).float(), draw(N, K).float(), draw(M, N).bfloat16()
+    xi, wi = ops.e4m3_rows(x), ops.e4m3_rows(w)
+    y, bits = ops.linear_e4m3(*xi, *wi, None, K, True, torch.bfloat16, True)
+    for rows in (slice(0, 100), slice(M // 2, M // 2 + 100), slice(M - 100, M)):
+        want = (x[rows] @ w.t()).relu()
+        assert torch.equal(y[rows], want.bfloat16())
+        assert np.array_equal(bits[rows].cpu().numpy(), O.pack_bits((want > 0).cpu().numpy()))
+    dX, dW, db = ops.linear_e4m3_backward(dy, bits, *xi, *wi, K)
+    want_dW, want_db = torch.zeros(N, K, dtype=torch.float64, device=dev), torch.zeros(N, dtype=torch.float64, device=dev)
+    for r in range(0, M, 100000):
+        dz = (dy[r:r + 100000] * (y[r:r + 100000] > 0)).double()
+        want_dW += dz.t().contiguous() @ x[r:r + 100000].double()
+        want_db += dz.sum(0)
+        assert torch.equal(dX[r:r + 100000], (dz.float() @ w).bfloat16())
+    assert torch.equal(dW.double(), want_dW) and torch.equal(db.double(), want_db)

@@ -164,3 +164,35 @@ def test_rows_of_a_wider_tensor(dev, dtype, N, E):
     part.copy_(d_out)
     grad = ops.embedding_rows_grad(part, tokens.to(dev), V, 1.0, torch.float32)
     assert torch.equal(grad.cpu(), torch.from_numpy(O.embedding_grad(_np(d_out), tokens.numpy(), V, 1.0)).float())
+
+
+def test_counts_past_the_abis_ints_are_refused(dev):
+    """Numbers of rows, tokens and table rows that a C int does not hold are refused before anything is allocated for them."""
+    from phonlp_amd import ops
+    tall = torch.empty(2 ** 31, 1, dtype=torch.float16, device=dev)
+    with pytest.raises(ValueError, match="more than"):
+        ops.e4m3_rows(tall)
+    with pytest.raises(ValueError, match="more than"):
+        ops.embedding_rows(tall, torch.zeros(1, dtype=torch.int64, device=dev))
+    with pytest.raises(ValueError, match="V must lie"):
+        ops.embedding_rows_grad(torch.ones(1, 4, device=dev), torch.zeros(1, dtype=torch.int64, device=dev), 2 ** 32 + 3)
+
+
+def test_tables_past_32_bit_offsets(dev):
+    """A table of more than 2^31 entries: its last rows are found, their gradients land there, every other row is zero."""
+    from phonlp_amd import ops
+    V, E = 2_900_000, 768
+    assert V * E > 2 ** 31
+    tokens = torch.tensor([V - 1, 5, V - 2, V - 1, V, V // 2], device=dev)
+    table = torch.zeros(V, E, dtype=torch.bfloat16, device=dev)
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randint(-9, 10, (6, E), generator=g).to(dev, torch.bfloat16)
+    table[tokens[[0, 1, 2, 5]]] = rows[:4]
+    out = ops.embedding_rows(table, tokens, 2.0)
+    assert torch.equal(out[[0, 1, 2, 5]], 2 * rows[:4]) and torch.equal(out[3], out[0]) and not out[4].any()
+    del table
+    d = ops.embedding_rows_grad(rows, tokens, V)
+    assert torch.equal(d[V - 1], rows[0] + rows[3]) and torch.equal(d[5], rows[1]) and torch.equal(d[V - 2], rows[2])
+    assert torch.equal(d[V // 2], rows[5])
+    d[tokens[[0, 1, 2, 5]]] = 0
+    assert not d.any()
