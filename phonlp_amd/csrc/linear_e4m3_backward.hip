@@ -8,7 +8,7 @@
 #include <type_traits>
 
 #include "e4m3.h"
-#include "tile128.h"
+#include "lds_dma.h"
 
 namespace phonlp {
 
