@@ -1,7 +1,7 @@
 // Embedding lookup with scaling, out[n] = scale * table[token_n], and its gradient by sorted tokens,
 // d_table[v] = scale * sum over the n with token_n = v of d_out[n]  (a token outside [0, V): a zero row, no gradient).
 //
-// The gradient sorts (token, n) stably, so that a token's rows stand together in ascending n; one wave sums the rows of a fixed
+// Up to 128 tokens each row of the table looks for its own.  Beyond, the gradient sorts (token, n) stably, so that a token's rows stand together in ascending n; one wave sums the rows of a fixed
 // number of sorted places and writes the runs of equal tokens that lie inside, runs that reach over a border leave fp32 shares
 // that a second launch adds in order.  No float atomics: the result does not depend on the launch, and a token that holds a large
 // share of all places is summed by as many waves as its places fill.  Both directions are bound by memory.
@@ -17,39 +17,35 @@ __device__ __forceinline__ int token_key(const I *tokens, long n, int V) {  // V
     return t >= 0 && t < (I)V ? (int)t : V;
 }
 
+// A lane takes VEC <= E neighbouring columns of a row; one that would reach behind the row's end takes its last VEC, some of them with its
+// neighbour, and both then hold and write the same values.  (A branch for every column of every row takes longer than the loads: 512 rows
+// on one wave, eight columns of bf16 a lane, 247 us against 121.)
+//
 // A wave takes sixteen tokens and a slab of 64 * VEC columns (blockIdx.y): one load for the tokens, a lane each, sixteen rows in flight.
 // Lanes behind a row's end stay with the others: the tokens are read from all sixteen lanes.
-template <class T, class I>
+template <int VEC, class T, class I>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(const T *table, long ld, const I *tokens, int N, int V, int E, float scale,
                                                              T *out) {
-    constexpr int VEC = 16 / sizeof(T), ROWS = 16;
+    constexpr int ROWS = 16;
     typedef typename Vec<T, VEC>::type Vt;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
-              left = E - from, col = E < VEC ? from : min(from, E - VEC);  // at a row's end some columns twice, the same values
+              col = min(from, E - VEC);  // at a row's end some columns twice, the same values
     const long n0 = (blockIdx.x * 4L + wave) * ROWS;
     if (n0 >= N) return;  // the whole wave
     const int rows = (int)min((long)ROWS, N - n0), held = token_key(tokens, n0 + min(lane, rows - 1), V);
     int key[ROWS];
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) key[u] = __builtin_amdgcn_readlane(held, u);
-    if (E >= VEC) {
-        if (left <= 0) return;
-        Vt v[ROWS];
+    if (from >= E) return;
+    Vt v[ROWS];
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) v[u] = *reinterpret_cast<const Vt *>(table + (key[u] < V ? key[u] : 0) * ld + col);
+    for (int u = 0; u < ROWS; ++u) v[u] = *reinterpret_cast<const Vt *>(table + (key[u] < V ? key[u] : 0) * ld + col);
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            Vt o;
+    for (int u = 0; u < ROWS; ++u) {
+        Vt o;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = key[u] < V ? (T)((float)v[u][i] * scale) : (T)0.f;
-            if (u < rows) *reinterpret_cast<Vt *>(out + (n0 + u) * E + col) = o;
-        }
-    } else if (left > 0) {
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u)
-            if (u < rows)
-                for (int i = 0; i < left; ++i)
-                    out[(n0 + u) * E + col + i] = key[u] < V ? (T)((float)table[key[u] * ld + col + i] * scale) : (T)0.f;
+        for (int i = 0; i < VEC; ++i) o[i] = key[u] < V ? (T)((float)v[u][i] * scale) : (T)0.f;
+        if (u < rows) *reinterpret_cast<Vt *>(out + (n0 + u) * E + col) = o;
     }
 }
 
@@ -226,32 +222,12 @@ __device__ __forceinline__ int lower_bound_wave(const int *sorted, int n, int ke
     return lo;
 }
 
-// A lane's VEC columns of a row, from `col`; `left` of them are there.  WHOLE: E >= VEC, and a lane that would reach behind the row takes
-// its last VEC columns, some of them with its neighbour, which then both hold the same sums, and a lane behind it reads without need.
-// (A branch for every column of every row takes longer than the loads: 512 rows on one wave, eight columns of bf16 a lane, 247 us
-// against 121.)
-template <bool WHOLE, class T, int VEC>
-__device__ __forceinline__ typename Vec<T, VEC>::type load_raw(const T *row, int col, int left) {
-    typedef typename Vec<T, VEC>::type Vt;
-    if (WHOLE || left >= VEC) return *reinterpret_cast<const Vt *>(row + col);
-    Vt v;
+template <class TO, int VEC>
+__device__ __forceinline__ void store_row(TO *p, const float (&v)[VEC], float scale) {
+    typename Vec<TO, VEC>::type t;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = i < left ? row[col + i] : (T)0.f;
-    return v;
-}
-template <bool WHOLE, class TO, int VEC>
-__device__ __forceinline__ void store_row(TO *p, int left, const float (&v)[VEC], float scale) {
-    typedef typename Vec<TO, VEC>::type Vt;
-    if (WHOLE ? left > 0 : left >= VEC) {
-        Vt t;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) t[i] = (TO)(v[i] * scale);
-        *reinterpret_cast<Vt *>(p) = t;
-    } else if (!WHOLE) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (i < left) p[i] = (TO)(v[i] * scale);
-    }
+    for (int i = 0; i < VEC; ++i) t[i] = (TO)(v[i] * scale);
+    *reinterpret_cast<typename Vec<TO, VEC>::type *>(p) = t;
 }
 
 struct SumArgs {
@@ -264,12 +240,58 @@ struct SumArgs {
     float scale;
 };
 
+// Few tokens, no sort: a wave owns up to 16 rows of the table (few, where the table is small: a row's tokens come one row after the other)
+// and a slab of columns, finds their tokens among all of them (two a lane) and adds the rows in ascending n, or writes zeros.  One launch
+// in place of three: 64000 x 768 bf16, 37 tokens 16.9 us against 20.6 by sorted tokens, 128 tokens 18.6 against 21.8; 24 x 100 fp32, 64
+// tokens 3.4 against 10.1; 128 times the same token of 1000 x 768 bf16 17.3 against 13.0.
+constexpr int kFewMost = 128;
+template <int VEC, class T, class TO, class I>
+__global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld, const I *tokens, int N, int V, int E, int rows, float scale, TO *table) {
+    constexpr int UNROLL = 16;
+    typedef typename Vec<T, VEC>::type Vt;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
+              col = min(from, E - VEC);
+    const long row0 = (blockIdx.x * 4L + wave) * rows;
+    if (row0 >= V) return;  // the whole wave
+    int at[2];  // which of the rows, for tokens lane and 64 + lane
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int n = h * 64 + lane, key = token_key(tokens, min(n, N - 1), V);
+        const long r = key - row0;
+        at[h] = n < N && key < V && r >= 0 && r < rows ? (int)r : -1;
+    }
+    for (int r = 0; r < rows && row0 + r < V; ++r) {
+        unsigned long long low = __ballot(at[0] == r), high = __ballot(at[1] == r);
+        float s[VEC] = {};
+        while (low | high) {
+            int n[UNROLL], count = 0;
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const bool more = low | high;
+                const unsigned long long m = low ? low : high, rest = m & (m - 1);
+                n[u] = more ? (low ? 0 : 64) + __ffsll(m) - 1 : n[u ? u - 1 : 0];
+                high = low ? high : rest;
+                low = low ? rest : 0;
+                count += more;
+            }
+            Vt v[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) v[u] = *reinterpret_cast<const Vt *>(d + n[u] * ld + col);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[i] += u < count ? (float)v[u][i] : 0.f;
+        }
+        if (from < E) store_row<TO, VEC>(table + (row0 + r) * E + col, s, scale);
+    }
+}
+
 // blockIdx.y: a slab of 64 * VEC columns.  blockIdx.x < sum_blocks: a wave per chunk of R sorted places, sixteen rows in flight; behind
 // them (first slab only): a wave per 16 rows of the table, which writes zeros where no token points (64 tokens, 64000 x 768
 // bf16: 22.3 us with a search per row, 21.2 with one per 16).
-template <class T, class TO>
+template <int VEC, class T, class TO>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
-    constexpr int VEC = 16 / sizeof(T), UNROLL = 16;
+    constexpr int UNROLL = 16;
     typedef typename Vec<T, VEC>::type Vt;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TO *table = (TO *)a.d_table;
@@ -291,59 +313,54 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
             }
             rows &= ~__ballot(there);
         }
-        constexpr int VO = 16 / sizeof(TO);
-        const float zero[VO] = {};
+        const float zero[VEC] = {};
         while (rows) {
             const int r = __ffsll(rows) - 1;
             rows &= rows - 1;
-            for (int c = lane * VO; c < a.E; c += 64 * VO) store_row<false, TO, VO>(table + (row0 + r) * a.E + c, a.E - c, zero, 0.f);
+            for (int c = lane * VEC; c < a.E; c += 64 * VEC) store_row<TO, VEC>(table + (row0 + r) * a.E + min(c, a.E - VEC), zero, 0.f);
         }
         return;
     }
-    const int chunk = blockIdx.x * 4 + wave, from = (blockIdx.y * 64 + lane) * VEC, left = a.E - from, col = a.E < VEC ? from : min(from, a.E - VEC);
+    const int chunk = blockIdx.x * 4 + wave, from = (blockIdx.y * 64 + lane) * VEC, col = min(from, a.E - VEC);
     if (chunk >= a.chunks) return;
     const int first = chunk * a.R, last = min(first + a.R, a.N);
     const T *d = (const T *)a.d_out;
-    auto sum = [&](auto w) {
-        constexpr bool WHOLE = decltype(w)::value;
-        bool head = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
-        float s[VEC] = {};
-        for (int p = first; p < last; p += UNROLL) {
-            // lane u holds place p + u
-            const int at = p + lane, row = a.order[min(at, last - 1)], key = at < a.N ? a.sorted[at] : -1;
-            Vt v[UNROLL];
+    bool head = first > 0 && a.sorted[first - 1] == a.sorted[first];  // the first run began before
+    float s[VEC] = {};
+    for (int p = first; p < last; p += UNROLL) {
+        // lane u holds place p + u
+        const int at = p + lane, row = a.order[min(at, last - 1)], key = at < a.N ? a.sorted[at] : -1;
+        Vt v[UNROLL];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) v[u] = load_raw<WHOLE, T, VEC>(d + (long)__builtin_amdgcn_readlane(row, u) * a.ld, col, left);
+        for (int u = 0; u < UNROLL; ++u) v[u] = *reinterpret_cast<const Vt *>(d + (long)__builtin_amdgcn_readlane(row, u) * a.ld + col);
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                if (p + u >= last) break;
+        for (int u = 0; u < UNROLL; ++u) {
+            if (p + u >= last) break;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) s[i] += (float)v[u][i];
-                const int k = __builtin_amdgcn_readlane(key, u);
-                const bool ends = __builtin_amdgcn_readlane(key, u + 1) != k;
-                if (!ends && p + u + 1 < last) continue;
-                if (k < a.V) {
-                    if (ends && !head) store_row<WHOLE, TO, VEC>(table + (long)k * a.E + col, left, s, a.scale);
-                    else store_row<WHOLE, float, VEC>(a.shares + ((long)chunk * 2 + (head ? 0 : 1)) * a.E + col, left, s, 1.f);
-                }
-                head = false;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+            for (int i = 0; i < VEC; ++i) s[i] += (float)v[u][i];
+            const int k = __builtin_amdgcn_readlane(key, u);
+            const bool ends = __builtin_amdgcn_readlane(key, u + 1) != k;
+            if (!ends && p + u + 1 < last) continue;
+            if (from < a.E && k < a.V) {
+                if (ends && !head) store_row<TO, VEC>(table + (long)k * a.E + col, s, a.scale);
+                else store_row<float, VEC>(a.shares + ((long)chunk * 2 + (head ? 0 : 1)) * a.E + col, s, 1.f);
             }
+            head = false;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s[i] = 0.f;
         }
-    };
-    if (a.E >= VEC) sum(std::true_type{});
-    else sum(std::false_type{});
+    }
 }
 
 // Runs that go on behind the chunk they begin in: their shares, in order.  A workgroup looks at eight chunks, a chunk per lane; runs of
 // up to 17 shares are summed by a wave each, longer ones by all eight waves, an eighth of the shares each.
-template <class T, class TO>
+template <int VEC, class TO>
 __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
-    constexpr int VEC = 16 / sizeof(T), UNROLL = 16 / (VEC / 4), FEW = 16;
+    constexpr int UNROLL = VEC == 8 ? 8 : 16, FEW = 16;
     __shared__ float sums[8][64 * VEC];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
-              left = a.E - from, col = a.E < VEC ? from : min(from, a.E - VEC), mine = blockIdx.x * 8 + lane;
+              col = min(from, a.E - VEC), mine = blockIdx.x * 8 + lane;
+    const bool in = from < a.E;
     auto reaches = [&](int chunk, int k) {  // the first place of `chunk` still holds k
         const long p = (long)chunk * a.R;
         return (p < a.N) & (a.sorted[min(p, (long)a.N - 1)] == k);
@@ -358,13 +375,14 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
             for (int i = 2; i <= FEW; ++i) count += reaches(mine + i, k);
         }
     }
-    auto add_as = [&](auto w, int chunk, int lo, int hi, float (&s)[VEC]) {
+    auto add = [&](int chunk, int lo, int hi, float (&s)[VEC]) {  // shares lo .. hi - 1: the chunk's last run, then the next chunks' first
         for (int c = lo; c < hi; c += UNROLL) {
-            typename Vec<float, VEC>::type v[UNROLL];
+            typedef typename Vec<float, VEC>::type Vf;
+            Vf v[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int k = min(c + u, hi - 1);
-                v[u] = load_raw<decltype(w)::value, float, VEC>(a.shares + ((long)(chunk + k) * 2 + (k ? 0 : 1)) * a.E, col, left);
+                v[u] = *reinterpret_cast<const Vf *>(a.shares + ((long)(chunk + k) * 2 + (k ? 0 : 1)) * a.E + col);
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u)
@@ -373,15 +391,7 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
                     if (c + u < hi) s[i] += v[u][i];
         }
     };
-    auto add = [&](int chunk, int lo, int hi, float (&s)[VEC]) {  // shares lo .. hi - 1: the chunk's last run, then the next chunks' first
-        if (a.E >= VEC) add_as(std::true_type{}, chunk, lo, hi, s);
-        else add_as(std::false_type{}, chunk, lo, hi, s);
-    };
-    auto store = [&](int k, const float (&s)[VEC]) {
-        TO *p = (TO *)a.d_table + (long)k * a.E + col;
-        if (a.E >= VEC) store_row<true, TO, VEC>(p, left, s, a.scale);
-        else store_row<false, TO, VEC>(p, left, s, a.scale);
-    };
+    auto store = [&](int k, const float (&s)[VEC]) { store_row<TO, VEC>((TO *)a.d_table + (long)k * a.E + col, s, a.scale); };
     int turn = 0;
     for (unsigned long long runs = __ballot(key < a.V); runs; runs &= runs - 1) {
         const int l = __ffsll(runs) - 1, chunk = blockIdx.x * 8 + l, k = __builtin_amdgcn_readlane(key, l);
@@ -392,18 +402,18 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
         }
         float s[VEC] = {};
         if (n <= FEW + 1) {
-            if ((turn++ & 7) == wave && left > 0) {
+            if ((turn++ & 7) == wave && in) {
                 add(chunk, 0, n, s);
                 store(k, s);
             }
             continue;
         }
         const int per = ceil_div(n, 8);
-        if (left > 0) add(chunk, wave * per, min(wave * per + per, n), s);
+        if (in) add(chunk, wave * per, min(wave * per + per, n), s);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sums[wave][i * 64 + lane] = s[i];
         __syncthreads();
-        if (wave == 0 && left > 0) {
+        if (wave == 0 && in) {
 #pragma unroll
             for (int w = 1; w < 8; ++w)
 #pragma unroll
@@ -461,20 +471,36 @@ static int sort_tokens(const I *tokens, int N, int V, const EmbeddingPlan &pl, c
     return PHONLP_OK;
 }
 
-template <class T, class TO>
+template <int VEC, class T, class TO>
 static int sum_rows(SumArgs a, hipStream_t st) {
-    constexpr int VEC = 16 / sizeof(T);
     const int slabs = ceil_div(a.E, 64 * VEC);
     a.sum_blocks = ceil_div(a.chunks, 4);
     {
         ProfScope ps("embedding_sum", st);
-        hipLaunchKernelGGL((embedding_sum_kernel<T, TO>), dim3(a.sum_blocks + ceil_div(a.V, 64), slabs), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((embedding_sum_kernel<VEC, T, TO>), dim3(a.sum_blocks + ceil_div(a.V, 64), slabs), dim3(256), 0, st, a);
         const int rc = check_launch("embedding_sum_kernel");
         if (rc || a.chunks == 1) return rc;
     }
     ProfScope ps("embedding_join", st);
-    hipLaunchKernelGGL((embedding_join_kernel<T, TO>), dim3(ceil_div(a.chunks - 1, 8), slabs), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((embedding_join_kernel<VEC, TO>), dim3(ceil_div(a.chunks - 1, 8), slabs), dim3(512), 0, st, a);
     return check_launch("embedding_join_kernel");
+}
+
+template <int VEC, class T, class TO, class I>
+static int few_rows(const SumArgs &a, const I *tokens, hipStream_t st) {
+    ProfScope ps("embedding_few", st);
+    const int rows = a.V >= 65536 ? 16 : ceil_div(a.V, 4096);  // of a wave: some 4096 waves a slab
+    hipLaunchKernelGGL((embedding_few_kernel<VEC, T, TO, I>), dim3(ceil_div(ceil_div(a.V, rows), 4), ceil_div(a.E, 64 * VEC)), dim3(256), 0,
+                       st, (const T *)a.d_out, a.ld, tokens, a.N, a.V, a.E, rows, a.scale, (TO *)a.d_table);
+    return check_launch("embedding_few_kernel");
+}
+
+// Calls f with the widest vector of T (16 bytes, 4 elements or one) that a row of E holds.
+template <class T, class F>
+static int with_vec(int E, F &&f) {
+    if (E >= 16 / (int)sizeof(T)) return f(std::integral_constant<int, 16 / (int)sizeof(T)>{});
+    if (E >= 4) return f(std::integral_constant<int, 4>{});
+    return f(std::integral_constant<int, 1>{});
 }
 
 }  // namespace phonlp
@@ -492,15 +518,17 @@ extern "C" int phonlp_embedding_rows(const void *table, int type, long ld, const
     ProfScope ps("embedding_rows", st);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        constexpr int VEC = 16 / sizeof(T);
-        const dim3 grid(ceil_div(ceil_div(N, 16), 4), ceil_div(E, 64 * VEC));
-        if (tokens_are_int64)
-            hipLaunchKernelGGL((embedding_rows_kernel<T, long>), grid, dim3(256), 0, st, (const T *)table, ld, (const long *)tokens, N, V, E,
-                               scale, (T *)out);
-        else
-            hipLaunchKernelGGL((embedding_rows_kernel<T, int>), grid, dim3(256), 0, st, (const T *)table, ld, (const int *)tokens, N, V, E,
-                               scale, (T *)out);
-        return check_launch("embedding_rows_kernel");
+        return with_vec<T>(E, [&](auto vec) {
+            constexpr int VEC = decltype(vec)::value;
+            const dim3 grid(ceil_div(ceil_div(N, 16), 4), ceil_div(E, 64 * VEC));
+            if (tokens_are_int64)
+                hipLaunchKernelGGL((embedding_rows_kernel<VEC, T, long>), grid, dim3(256), 0, st, (const T *)table, ld, (const long *)tokens, N,
+                                   V, E, scale, (T *)out);
+            else
+                hipLaunchKernelGGL((embedding_rows_kernel<VEC, T, int>), grid, dim3(256), 0, st, (const T *)table, ld, (const int *)tokens, N,
+                                   V, E, scale, (T *)out);
+            return check_launch("embedding_rows_kernel");
+        });
     });
 }
 
@@ -519,15 +547,27 @@ extern "C" int phonlp_embedding_rows_grad(const void *d_out, int type, long ld, 
         return fail(PHONLP_ERR_WORKSPACE, "embedding_rows_grad: workspace too small or not 16-byte aligned");
     hipStream_t st = as_stream(stream);
     const EmbeddingPlan pl = plan_embedding(N, E);
-    const bool radix = N > kPlaceMost;
-    int *order, *sorted;
-    const int rc = tokens_are_int64 ? sort_tokens((const long *)tokens, N, V, pl, (char *)ws, &order, &sorted, st)
-                                    : sort_tokens((const int *)tokens, N, V, pl, (char *)ws, &order, &sorted, st);
-    if (rc) return rc;
-    SumArgs a = {d_out, d_table, (float *)((char *)ws + pl.pairs * (radix ? 4 : 2)), order, sorted, ld, N, V, E, pl.R, pl.chunks, 0, scale};
+    SumArgs a = {d_out, d_table, nullptr, nullptr, nullptr, ld, N, V, E, pl.R, pl.chunks, 0, scale};
+    const bool few = N <= kFewMost, radix = N > kPlaceMost;
+    if (!few) {
+        int *order, *sorted;
+        const int rc = tokens_are_int64 ? sort_tokens((const long *)tokens, N, V, pl, (char *)ws, &order, &sorted, st)
+                                        : sort_tokens((const int *)tokens, N, V, pl, (char *)ws, &order, &sorted, st);
+        if (rc) return rc;
+        a.order = order;
+        a.sorted = sorted;
+        a.shares = (float *)((char *)ws + pl.pairs * (radix ? 4 : 2));
+    }
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (table_type == PHONLP_F32) return sum_rows<T, float>(a, st);
-        return sum_rows<T, T>(a, st);
+        return with_vec<T>(E, [&](auto vec) {
+            constexpr int VEC = decltype(vec)::value;
+            auto run = [&](auto to) {
+                using TO = decltype(to);
+                if (!few) return sum_rows<VEC, T, TO>(a, st);
+                return tokens_are_int64 ? few_rows<VEC, T, TO>(a, (const long *)tokens, st) : few_rows<VEC, T, TO>(a, (const int *)tokens, st);
+            };
+            return table_type == PHONLP_F32 ? run(float{}) : run(T{});
+        });
     });
 }

@@ -196,3 +196,21 @@ def test_tables_past_32_bit_offsets(dev):
     assert torch.equal(d[V // 2], rows[5])
     d[tokens[[0, 1, 2, 5]]] = 0
     assert not d.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("N", [2, 63, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("V,E,spread", [(3, 5, "zipf"), (4097, 12, "outside"), (9000, 300, "even"), (70001, 2, "one"), (140000, 9, "outside")])
+def test_few_tokens(dev, dtype, N, V, E, spread):
+    """Both sides of the border between looking for a row's tokens and sorting them; one to sixteen rows of the table a wave; more tokens
+    of a row than are loaded at a time.  Whole numbers: exact, and the same twice."""
+    from phonlp_amd import ops
+    g = torch.Generator().manual_seed(N + V)
+    tokens = _tokens(g, N, V, spread)
+    d_out = torch.randint(-7, 8, (N, E), generator=g).to(dtype)
+    want = torch.from_numpy(O.embedding_grad(_np(d_out), tokens.numpy(), V, 0.5)).float()
+    for kind in (torch.int64, torch.int32):
+        t = tokens.to(kind).to(dev)
+        grad = ops.embedding_rows_grad(d_out.to(dev), t, V, 0.5, torch.float32)
+        assert torch.equal(grad.cpu(), want)
+        assert torch.equal(ops.embedding_rows_grad(d_out.to(dev), t, V, 0.5).cpu(), want.to(dtype))
