@@ -1,10 +1,11 @@
 // Embedding lookup with scaling, out[n] = scale * table[token_n], and its gradient by sorted tokens,
 // d_table[v] = scale * sum over the n with token_n = v of d_out[n]  (a token outside [0, V): a zero row, no gradient).
 //
-// Up to 128 tokens each row of the table looks for its own.  Beyond, the gradient sorts (token, n) stably, so that a token's rows stand together in ascending n; one wave sums the rows of a fixed
-// number of sorted places and writes the runs of equal tokens that lie inside, runs that reach over a border leave fp32 shares
-// that a second launch adds in order.  No float atomics: the result does not depend on the launch, and a token that holds a large
-// share of all places is summed by as many waves as its places fill.  Both directions are bound by memory.
+// Up to kFewMost tokens each row of the table looks for its own.  Beyond, the gradient sorts (token, n) stably, so that a token's rows
+// stand together in ascending n; one wave sums the rows of a fixed number of sorted places and writes the runs of equal tokens that lie
+// inside, runs that reach over a border leave fp32 shares that a second launch adds in order.  No float atomics: the result does not
+// depend on the launch, and a token that holds a large share of all places is summed by as many waves as its places fill.  Both
+// directions are bound by memory.
 #include <type_traits>
 
 #include "e4m3.h"
@@ -240,39 +241,53 @@ struct SumArgs {
     float scale;
 };
 
-// Few tokens, no sort: a wave owns up to 16 rows of the table (few, where the table is small: a row's tokens come one row after the other)
-// and a slab of columns, finds their tokens among all of them (two a lane) and adds the rows in ascending n, or writes zeros.  One launch
-// in place of three: 64000 x 768 bf16, 37 tokens 16.9 us against 20.6 by sorted tokens, 128 tokens 18.6 against 21.8; 24 x 100 fp32, 64
-// tokens 3.4 against 10.1; 128 times the same token of 1000 x 768 bf16 17.3 against 13.0.
-constexpr int kFewMost = 128;
+// Few tokens, no sort: a workgroup owns `rows` <= 64 rows of the table (few, where the table is small: a row's tokens come one after the
+// other) and a slab of columns.  Each of its four waves takes a quarter of the tokens, two a lane at most, and adds those of a row in
+// ascending n; a row that several waves have tokens of is the sum of their shares in ascending order, one without tokens is zeros.
+// One launch in place of three: 64000 x 768 bf16, 37 tokens 16.6 us against 20.3 by sorted tokens, 512 tokens 19.3 against 22.5; 24 x 100
+// fp32, 512 tokens 4.2 against 13.5; at worst, 512 times the same token of 1000 x 768 bf16, 30 against 15.
+constexpr int kFewMost = 512;
 template <int VEC, class T, class TO, class I>
 __global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld, const I *tokens, int N, int V, int E, int rows, float scale, TO *table) {
     constexpr int UNROLL = 16;
     typedef typename Vec<T, VEC>::type Vt;
+    __shared__ float shares[4][64 * VEC];
+    __shared__ unsigned there[4][2];  // of each wave, the rows that it has tokens of
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
-              col = min(from, E - VEC);
-    const long row0 = (blockIdx.x * 4L + wave) * rows;
-    if (row0 >= V) return;  // the whole wave
-    int at[2];  // which of the rows, for tokens lane and 64 + lane
+              col = min(from, E - VEC), each = ceil_div(N, 4), first = wave * each, mine = min(each, N - first);
+    const long row0 = (long)blockIdx.x * rows;
+    const int have = (int)min((long)rows, V - row0);
+    if (threadIdx.x < 8) there[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    __syncthreads();
+    int at[2];  // which of the rows, for this wave's tokens lane and 64 + lane
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int n = h * 64 + lane, key = token_key(tokens, min(n, N - 1), V);
+        const int n = h * 64 + lane, key = token_key(tokens, min(first + n, N - 1), V);
         const long r = key - row0;
-        at[h] = n < N && key < V && r >= 0 && r < rows ? (int)r : -1;
+        at[h] = n < mine && key < V && r >= 0 && r < have ? (int)r : -1;
+        if (at[h] >= 0) atomicOr(&there[wave][at[h] >> 5], 1u << (at[h] & 31));
     }
-    for (int r = 0; r < rows && row0 + r < V; ++r) {
+    __syncthreads();
+    unsigned long long one = 0, more = 0, own = 0;  // rows with tokens of one wave or more, of two or more, of this one
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const unsigned long long m = there[w][0] | (unsigned long long)there[w][1] << 32;
+        more |= one & m;
+        one |= m;
+        if (w == wave) own = m;
+    }
+    auto add = [&](int r, float (&s)[VEC]) {  // this wave's rows of token row0 + r
         unsigned long long low = __ballot(at[0] == r), high = __ballot(at[1] == r);
-        float s[VEC] = {};
         while (low | high) {
             int n[UNROLL], count = 0;
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                const bool more = low | high;
+                const bool any = low | high;
                 const unsigned long long m = low ? low : high, rest = m & (m - 1);
-                n[u] = more ? (low ? 0 : 64) + __ffsll(m) - 1 : n[u ? u - 1 : 0];
+                n[u] = any ? first + (low ? 0 : 64) + __ffsll(m) - 1 : n[u ? u - 1 : 0];
                 high = low ? high : rest;
                 low = low ? rest : 0;
-                count += more;
+                count += any;
             }
             Vt v[UNROLL];
 #pragma unroll
@@ -282,7 +297,35 @@ __global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld,
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) s[i] += u < count ? (float)v[u][i] : 0.f;
         }
-        if (from < E) store_row<TO, VEC>(table + (row0 + r) * E + col, s, scale);
+    };
+    TO *out = table + row0 * E + col;
+    const bool in = from < E;
+    if (in) {
+        const float zero[VEC] = {};
+        for (unsigned long long rest = ~one & (~0ull >> (64 - have)) & 0x1111111111111111ull << wave; rest; rest &= rest - 1)
+            store_row<TO, VEC>(out + (long)(__ffsll(rest) - 1) * E, zero, 0.f);
+    }
+    for (unsigned long long rest = own & ~more; rest; rest &= rest - 1) {
+        const int r = __ffsll(rest) - 1;
+        float s[VEC] = {};
+        add(r, s);
+        if (in) store_row<TO, VEC>(out + (long)r * E, s, scale);
+    }
+    for (unsigned long long rest = more; rest; rest &= rest - 1) {  // all four waves
+        const int r = __ffsll(rest) - 1;
+        float s[VEC] = {};
+        add(r, s);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) shares[wave][i * 64 + lane] = s[i];
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int w = 1; w < 4; ++w)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[i] += shares[w][i * 64 + lane];
+            if (in) store_row<TO, VEC>(out + (long)r * E, s, scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -489,8 +532,8 @@ static int sum_rows(SumArgs a, hipStream_t st) {
 template <int VEC, class T, class TO, class I>
 static int few_rows(const SumArgs &a, const I *tokens, hipStream_t st) {
     ProfScope ps("embedding_few", st);
-    const int rows = a.V >= 65536 ? 16 : ceil_div(a.V, 4096);  // of a wave: some 4096 waves a slab
-    hipLaunchKernelGGL((embedding_few_kernel<VEC, T, TO, I>), dim3(ceil_div(ceil_div(a.V, rows), 4), ceil_div(a.E, 64 * VEC)), dim3(256), 0,
+    const int rows = a.V >= 65536 ? 64 : ceil_div(a.V, 1024);  // of a workgroup: some thousand of them a slab
+    hipLaunchKernelGGL((embedding_few_kernel<VEC, T, TO, I>), dim3(ceil_div(a.V, rows), ceil_div(a.E, 64 * VEC)), dim3(256), 0,
                        st, (const T *)a.d_out, a.ld, tokens, a.N, a.V, a.E, rows, a.scale, (TO *)a.d_table);
     return check_launch("embedding_few_kernel");
 }

@@ -199,11 +199,11 @@ def test_tables_past_32_bit_offsets(dev):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
-@pytest.mark.parametrize("N", [2, 63, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("N", [2, 5, 63, 64, 65, 127, 129, 255, 511, 512, 513])
 @pytest.mark.parametrize("V,E,spread", [(3, 5, "zipf"), (4097, 12, "outside"), (9000, 300, "even"), (70001, 2, "one"), (140000, 9, "outside")])
 def test_few_tokens(dev, dtype, N, V, E, spread):
-    """Both sides of the border between looking for a row's tokens and sorting them; one to sixteen rows of the table a wave; more tokens
-    of a row than are loaded at a time.  Whole numbers: exact, and the same twice."""
+    """Both sides of the border between looking for a row's tokens and sorting them; one to 64 rows of the table a workgroup; tokens of one
+    wave and of several, more of a row than are loaded at a time.  Whole numbers: exact, and the same twice."""
     from phonlp_amd import ops
     g = torch.Generator().manual_seed(N + V)
     tokens = _tokens(g, N, V, spread)
