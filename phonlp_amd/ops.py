@@ -964,6 +964,15 @@ def _run(device, name, *args):
         check(rc, name)
 
 
+_PLAIN = {Tensor, torch.nn.Parameter}
+
+
+def _traced(t: Tensor) -> bool:
+    """A fake tensor, or a call that torch.compile traces: it goes through the registered op (below), which an eager call leaves out for
+    its host time."""
+    return type(t) not in _PLAIN or torch.compiler.is_compiling()
+
+
 def _new(rows: int, cols: int, dtype, device) -> Tensor:
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)  # a quarter less host time than torch.empty
 
@@ -1026,6 +1035,8 @@ def e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
     """x [rows, K] fp32 / bf16 / fp16 (row stride free, unit column stride) -> its e4m3 image: codes float8_e4m3fn
     [rows, e4m3_kp(K)], exponents uint8 [rows, e4m3_kb(K)] (one power-of-two scale per row and block of 128 columns; infinities and
     NaN become NaN).  The operand form of linear_e4m3, and a layer input's 8-bit checkpoint for linear_e4m3_backward."""
+    if _traced(x):
+        return torch.ops.phonlp_amd.e4m3_rows(x)
     code, ld, rows, K = _rows_of(x, "x")
     if K == 0:
         raise ValueError("e4m3_rows: x has no columns")
@@ -1039,6 +1050,8 @@ def e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
 
 def e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype = torch.float32) -> Tensor:
     """The values [rows, K] that an e4m3 image stands for: exact in fp32 and bf16, 16-bit types saturate at their largest."""
+    if _traced(codes):
+        return torch.ops.phonlp_amd.e4m3_values(codes, exponents, K, dtype)
     rows = _image_of(codes, exponents, K, "codes")
     if dtype not in _TYPES:
         raise ValueError(f"e4m3_values: dtype must be float32, bfloat16 or float16, got {dtype}")
@@ -1054,6 +1067,9 @@ def linear_e4m3(x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponen
     """y = act(x @ w.T + bias) on the e4m3 images of x [M, K] and w [N, K] (e4m3_rows) -> (y [M, N] in `dtype`, bits).
     bits (want_bits): int32 [M, ceil(N / 32)], bit n % 32 of word n / 32 set where y > 0 -- what linear_e4m3_backward needs of a
     ReLU layer; else None."""
+    if _traced(x_codes):
+        y, bits = torch.ops.phonlp_amd.linear_e4m3(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits)
+        return y, bits if want_bits else None
     M = _image_of(x_codes, x_exponents, K, "x_codes")
     N = _image_of(w_codes, w_exponents, K, "w_codes")
     dev = x_codes.device
@@ -1114,6 +1130,8 @@ def _tokens_of(tokens: Tensor, device) -> int:
 def embedding_rows(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
     """scale * table[tokens]: table [V, E] fp32 / bf16 / fp16 (row stride free), tokens int32 / int64 of any shape -> [*tokens.shape,
     E] of the table's type.  A token outside [0, V) gives a row of zeros."""
+    if _traced(table):
+        return torch.ops.phonlp_amd.embedding_rows(table, tokens, scale)
     code, ld, V, E = _rows_of(table, "table")
     N = _tokens_of(tokens, table.device)
     out = torch.empty((*tokens.shape, E), dtype=table.dtype, device=table.device)
@@ -1152,6 +1170,52 @@ def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.
     _run(dev, "phonlp_embedding_rows_grad", d_out.data_ptr(), code, ld, tokens.data_ptr(), int(tokens.dtype == torch.int64), N, V, E,
          float(scale), d_table.data_ptr(), _TYPES[dtype], ws.data_ptr(), max(nb, 256))
     return d_table
+
+
+# The forward ones as registered ops, for tracing; without bits linear_e4m3 returns an empty tensor in their place.
+@torch.library.custom_op("phonlp_amd::e4m3_rows", mutates_args=())
+def _e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
+    return e4m3_rows(x)
+
+
+@_e4m3_rows.register_fake
+def _(x):
+    rows, K = x.shape
+    return x.new_empty((rows, e4m3_kp(K)), dtype=_E4M3), x.new_empty((rows, e4m3_kb(K)), dtype=torch.uint8)
+
+
+@torch.library.custom_op("phonlp_amd::e4m3_values", mutates_args=())
+def _e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype) -> Tensor:
+    return e4m3_values(codes, exponents, K, dtype)
+
+
+@_e4m3_values.register_fake
+def _(codes, exponents, K, dtype):
+    return codes.new_empty((codes.shape[0], K), dtype=dtype)
+
+
+@torch.library.custom_op("phonlp_amd::linear_e4m3", mutates_args=())
+def _linear_e4m3(x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponents: Tensor, bias: Optional[Tensor], K: int, relu: bool,
+                 dtype: torch.dtype, want_bits: bool) -> Tuple[Tensor, Tensor]:
+    y, bits = linear_e4m3(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits)
+    return y, y.new_empty((0,), dtype=torch.int32) if bits is None else bits
+
+
+@_linear_e4m3.register_fake
+def _(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits):
+    M, N = x_codes.shape[0], w_codes.shape[0]
+    return (x_codes.new_empty((M, N), dtype=dtype),
+            x_codes.new_empty((M, (N + 31) // 32) if want_bits else (0,), dtype=torch.int32))
+
+
+@torch.library.custom_op("phonlp_amd::embedding_rows", mutates_args=())
+def _embedding_rows(table: Tensor, tokens: Tensor, scale: float) -> Tensor:
+    return embedding_rows(table, tokens, scale)
+
+
+@_embedding_rows.register_fake
+def _(table, tokens, scale):
+    return table.new_empty((*tokens.shape, table.shape[1]))
 
 
 # ---- shape functions (torch.library `register_fake`) for the ops above that had none: with them every custom op of

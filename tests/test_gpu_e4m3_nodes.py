@@ -353,3 +353,29 @@ def test_training_pass_on_8_bit_layers(dev, golden, monkeypatch, task):
     for k in want:
         off = float((grads[k] - want[k]).double().norm())
         assert off <= 2.0 ** -8 * float(want[k].double().norm()) + 1e-12, f"{k}: {off:.3e}"
+
+
+def test_registered_ops_are_the_functions(dev):
+    """torch.ops.phonlp_amd.* against the functions, results and what the shape functions promise."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from phonlp_amd import ops
+    R = torch.ops.phonlp_amd
+    g = torch.Generator().manual_seed(4)
+    x, w, b = torch.randn(9, 140, generator=g).to(dev), torch.randn(40, 140, generator=g).to(dev), torch.randn(40, generator=g).to(dev)
+    table, tokens = torch.randn(30, 24, generator=g).to(dev), torch.randint(-1, 31, (3, 5), generator=g).to(dev)
+    xi, wi = ops.e4m3_rows(x), ops.e4m3_rows(w)
+    calls = [(R.e4m3_rows, (x,), xi), (R.e4m3_values, (*xi, 140, torch.bfloat16), (ops.e4m3_values(*xi, 140, torch.bfloat16),)),
+             (R.linear_e4m3, (*xi, *wi, b, 140, True, torch.float32, True), ops.linear_e4m3(*xi, *wi, b, 140, True, torch.float32, True)),
+             (R.embedding_rows, (table, tokens, 0.5), (ops.embedding_rows(table, tokens, 0.5),))]
+    for op, args, want in calls:
+        got = op(*args)
+        got = got if isinstance(got, (tuple, list)) else (got,)
+        assert all(torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, c.view(torch.uint8) if c.element_size() == 1 else c)
+                   for a, c in zip(got, want))
+        with FakeTensorMode() as mode:
+            fake = op(*(mode.from_tensor(a) if isinstance(a, torch.Tensor) else a for a in args))
+        fake = fake if isinstance(fake, (tuple, list)) else (fake,)
+        assert [(f.shape, f.dtype) for f in fake] == [(a.shape, a.dtype) for a in got]
+    y, bits = R.linear_e4m3(*xi, *wi, None, 140, False, torch.float32, False)
+    assert bits.numel() == 0 and torch.equal(y, ops.linear_e4m3(*xi, *wi, None, 140, False)[0])
