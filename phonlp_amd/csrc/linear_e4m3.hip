@@ -355,78 +355,102 @@ __global__ __launch_bounds__(512) void linear_e4m3_kernel(E4m3Args a) {
     dma_wait<0>();  // the repeated loads still write this workgroup's LDS
 }
 
-// Few rows: a workgroup takes 32 x 32 of Y and its eight waves an eighth of the blocks each, straight from memory to registers (no
-// LDS but for the sum over the waves, which is in a fixed order); bound by reading W, or by latency.  Always the bf16 pipe.
-template <class T>
+// Few rows: straight from memory to registers, the next block's codes on their way while one is multiplied.  A workgroup takes 16 MF rows
+// of Y and 8 / KS groups of 32 columns; KS waves of a group take every KS-th block each, and their sums are added in a fixed order.  Bound
+// by reading W, or by latency.  Always the bf16 pipe.
+template <int MF, int KS, class T>
 __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(E4m3Args a) {
-    __shared__ float sums[8][32][33];
+    constexpr int GROUPS = 8 / KS;
+    __shared__ float sums[8][MF * 16][33];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32, blocks = a.Kp / 128;
-    f32x4 acc[2][2];
+    const int n0 = blockIdx.x * (32 * GROUPS), m0 = blockIdx.y * (16 * MF), blocks = a.Kp / 128, nw = n0 + wave / KS * 32;
+    f32x4 acc[MF][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    long xr[2], wr[2];
+    long xr[MF], wr[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        xr[i] = min(m0 + i * 16 + l16, a.M - 1);
-        wr[i] = min(n0 + i * 16 + l16, a.N - 1);
-    }
-    for (int kb = wave; kb < blocks; kb += 8) {
-        i32x4 x[2][2], w[2][2];  // 32 codes of a row per lane, from 32 g
-        float sx[2], sw[2];
+    for (int i = 0; i < MF; ++i) xr[i] = min(m0 + i * 16 + l16, a.M - 1);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int j = 0; j < 2; ++j) wr[j] = min(nw + j * 16 + l16, a.N - 1);
+    struct Block {  // 32 codes of a row per lane, from 32 g
+        i32x4 x[MF][2], w[2][2];
+        int ex[MF], ew[2];
+    };
+    auto load = [&](int kb, Block &b) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                x[i][h] = *reinterpret_cast<const i32x4 *>(a.x + xr[i] * a.Kp + kb * 128 + g * 32 + h * 16);
-                w[i][h] = *reinterpret_cast<const i32x4 *>(a.w + wr[i] * a.Kp + kb * 128 + g * 32 + h * 16);
-            }
-            sx[i] = scale_of(a.xe[xr[i] * a.KB4 + kb]);
-            sw[i] = scale_of(a.we[wr[i] * a.KB4 + kb]);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) b.w[j][h] = *reinterpret_cast<const i32x4 *>(a.w + wr[j] * a.Kp + kb * 128 + g * 32 + h * 16);
+#pragma unroll
+            for (int i = 0; i < MF; ++i) b.x[i][h] = *reinterpret_cast<const i32x4 *>(a.x + xr[i] * a.Kp + kb * 128 + g * 32 + h * 16);
         }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) b.ew[j] = a.we[wr[j] * a.KB4 + kb];
+#pragma unroll
+        for (int i = 0; i < MF; ++i) b.ex[i] = a.xe[xr[i] * a.KB4 + kb];
+    };
+    auto multiply = [&](const Block &b) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                bf16x8 fx[2], fw[2];
+                bf16x8 fx[MF], fw[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    fx[i] = widen(x[i][h][2 * q], x[i][h][2 * q + 1], sx[i]);
-                    fw[i] = widen(w[i][h][2 * q], w[i][h][2 * q + 1], sw[i]);
-                }
+                for (int i = 0; i < MF; ++i) fx[i] = widen(b.x[i][h][2 * q], b.x[i][h][2 * q + 1], scale_of(b.ex[i]));
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int j = 0; j < 2; ++j) fw[j] = widen(b.w[j][h][2 * q], b.w[j][h][2 * q + 1], scale_of(b.ew[j]));
+#pragma unroll
+                for (int i = 0; i < MF; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[i], fw[j], acc[i][j], 0, 0, 0);
             }
+    };
+    const int first = wave % KS;
+    if (first < blocks && nw < a.N) {
+        Block b0, b1;
+        load(first, b0);
+        for (int kb = first; kb < blocks; kb += 2 * KS) {  // two blocks a turn, so that each stands where it is
+            load(min(kb + KS, blocks - 1), b1);
+            multiply(b0);
+            if (kb + KS >= blocks) break;
+            load(min(kb + 2 * KS, blocks - 1), b0);
+            multiply(b1);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) sums[wave][i * 16 + g * 4 + r][j * 16 + l16] = acc[i][j][r];
     __syncthreads();
-    // 128 threads, eight columns of a row each: a byte of bits is one thread's
-    if (threadIdx.x >= 128) return;
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8, m = m0 + r, waves = min(8, blocks);
+    // eight columns of a row a thread: a byte of bits is one thread's
+    if (threadIdx.x >= MF * 16 * 4 * GROUPS) return;
+    const int u = threadIdx.x % (4 * GROUPS), group = u >> 2, r = threadIdx.x / (4 * GROUPS), c = (u & 3) * 8, m = m0 + r, nc = n0 + group * 32 + c,
+              waves = min(KS, blocks);
     if (m >= a.M) return;
     int b = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const int n = n0 + c + k;
+        const int n = nc + k;
         if (n >= a.N) continue;
         float v = 0.f;
-        for (int w = 0; w < waves; ++w) v += sums[w][r][c + k];
+        for (int w = 0; w < waves; ++w) v += sums[group * KS + w][r][c + k];
         if (a.bias) v += a.bias[n];
         if (a.relu) v = v < 0.f ? 0.f : v;  // keeps NaN
         const T t = (T)v;
         ((T *)a.y)[(long)m * a.N + n] = t;
         b |= (float)t > 0.f ? 1 << k : 0;
     }
-    if (a.bits && (n0 + c) >> 3 < a.row_bytes) a.bits[(long)m * a.row_bytes + ((n0 + c) >> 3)] = (uint8_t)b;
+    if (a.bits && nc >> 3 < a.row_bytes) a.bits[(long)m * a.row_bytes + (nc >> 3)] = (uint8_t)b;
+}
+
+template <int MF, int KS, class T>
+static int launch_few(const E4m3Args &a, hipStream_t st) {
+    hipLaunchKernelGGL((linear_e4m3_few_kernel<MF, KS, T>), dim3(ceil_div(a.N, 256 / KS), ceil_div(a.M, 16 * MF)), dim3(512), 0, st, a);
+    return check_launch("linear_e4m3_few_kernel");
 }
 
 template <int TM, int TN, class T>
@@ -480,13 +504,14 @@ extern "C" int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponent
     ProfScope ps("linear_e4m3", st);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        // Up to so many 32 x 32 the few-row form is the faster one; tiles of 128 x 128 would leave most compute units without work (fp32:
-        // 256 x 868 x 868 6.2 against 11.0 us, 256 x 2448 x 868, 616 of them, 10.8 against 11.3, 2048 x 400 x 768, 832, 11.9 against 10.6;
-        // 16-bit: 256 x 868 x 868 6.2 against 7.3, 128 x 2448 x 868, 308, 8.0 against 7.2)
-        if ((long)ceil_div(M, 32) * ceil_div(N, 32) <= (sizeof(T) == 4 ? 640 : 256)) {
-            hipLaunchKernelGGL((linear_e4m3_few_kernel<T>), dim3(ceil_div(N, 32), ceil_div(M, 32)), dim3(512), 0, st, a);
-            return check_launch("linear_e4m3_few_kernel");
-        }
+        // Up to sixteen rows, one token's among them, W is read once, at most of memory's rate: 1 x 64000 x 768 10.7 us (fp32 tiles of 128 x
+        // 128 18.9, 16-bit 12.3; 4.6 TB/s), 1 x 8192 x 8192 18 (60; 40), 1 x 28672 x 4096 26.5 (38.5; 24.8).  Two waves of a group where
+        // there are many groups: 10.7 against 12.3 with eight; 1 x 13464 x 4096 26 against 16.
+        if (M <= 16) return ceil_div(N, 32) > 640 ? launch_few<1, 2, T>(a, st) : launch_few<1, 8, T>(a, st);
+        // Of more rows, up to so many 32 x 32 the few-row form is the faster one; tiles of 128 x 128 would leave most compute units without
+        // work (fp32: 256 x 868 x 868 6.4 against 10.9 us, 256 x 2448 x 868, 616 of them, 10.8 against 11.3, 2048 x 400 x 768, 832, 11.9
+        // against 10.6; 16-bit: 256 x 868 x 868 6.3 against 7.3, 128 x 2448 x 868, 308, 8.0 against 7.2)
+        if ((long)ceil_div(M, 32) * ceil_div(N, 32) <= (sizeof(T) == 4 ? 640 : 256)) return launch_few<2, 8, T>(a, st);
         if (large_tile<T>(M, N, a.Kp)) return launch_tile<256, 256, T>(a, st);
         return launch_tile<128, 128, T>(a, st);
     });

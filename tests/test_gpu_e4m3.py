@@ -356,3 +356,21 @@ def test_products_past_32_bit_offsets(dev):
         want_db += dz.sum(0)
         assert torch.equal(dX[r:r + 100000], (dz.float() @ w).bfloat16())
     assert torch.equal(dW.double(), want_dW) and torch.equal(db.double(), want_db)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M", [1, 15, 16, 17])
+@pytest.mark.parametrize("N,K", [(20480, 700), (20481, 130), (30001, 1030), (1000, 128), (33, 3000)])
+def test_linear_few_rows(dev, dtype, M, N, K):
+    """One to seventeen rows: both groupings of the few-row form, one block to many, odd widths; whole numbers, exact."""
+    from phonlp_amd import ops
+    g = torch.Generator().manual_seed(N + M)
+    x, w, bias = (_whole(g, *s, 7).to(dev) for s in ((M, K), (N, K), (1, N)))
+    bias = bias[0].contiguous()
+    xi, wi = ops.e4m3_rows(x), ops.e4m3_rows(w)
+    want = (x.double() @ w.double().t() + bias.double()).relu()
+    y, bits = ops.linear_e4m3(*xi, *wi, bias, K, True, dtype, True)
+    assert torch.equal(y, want.to(dtype))
+    assert np.array_equal(bits.cpu().numpy(), O.pack_bits((want > 0).cpu().numpy()))
+    y, _ = ops.linear_e4m3(*xi, *wi, None, K, False, dtype)
+    assert torch.equal(y, (x.double() @ w.double().t()).to(dtype))
