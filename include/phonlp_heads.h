@@ -528,9 +528,8 @@ int phonlp_e4m3_values(const void *codes, const uint8_t *exponents, int rows, in
 
 /* Y[M,N] = act(X^ . W^^T + bias[N]) with X^, W^ the values of two images with the same K; fp32 sums, Y in `type`, row pitch N.
  * bias may be NULL.  relu: max(., 0), NaN kept.  bits: NULL, or [M, ceil(N / 32)] words with bit n % 32 of word n / 32 set where the
- * stored Y[m][n] > 0 (zero behind N) -- what the backward needs of a ReLU layer's output.  fp32 results are exact products added
- * in fp32; 16-bit results of larger products come from the 8-bit matrix pipe, which adds eight products cut off 13 bits below the
- * largest of them. */
+ * stored Y[m][n] > 0 (zero behind N) -- what the backward needs of a ReLU layer's output.  Products are exact, added in
+ * fp32 and rounded to `type` once. */
 int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents,
                        const float *bias, void *y, int type, uint32_t *bits, int M, int N, int K, int relu, void *stream);
 
