@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "e4m3.h"
+#include "e4m3_backward.h"
 #include "lds_dma.h"
 
 namespace phonlp {
@@ -163,9 +164,10 @@ __device__ __forceinline__ void store_quad(T *p, const f32x4 &v, int left) {
 // One of the two products,  C[i][j] = sum_p sum_r A_p(i, r) B[r][j]:  B the values of an image, bf16 rows r; A the pieces of dZ, for dX
 // with i their rows and r their columns, for dW with r their rows and i their columns.
 struct BwProduct {
-    const uint8_t *a, *b;  // [P][..][pitch_a bytes], [R up to 32][pitch_b bytes]
-    void *c;               // [I][J], or fp32 partial sums [S][I][J]
-    long pitch_a, plane, pitch_b;
+    BwOperand a;
+    const uint8_t *b;  // [R up to 32][pitch_b bytes]
+    void *c;           // [I][J], or fp32 partial sums [S][I][J]
+    long pitch_b;
     int I, J, R, num_i, num_j, per_split, splits, blocks;  // per_split: steps of 32 r
 };
 struct BwArgs {
@@ -176,10 +178,7 @@ struct BwArgs {
 };
 
 // LDS images.  Of a tile whose reduction runs along its rows, [i][32 r], 64 bytes a row: chunk c (16 bytes) of row i at slot
-// c ^ ((i >> 2) & 3), so that the chunks c of sixteen rows lie in all 64 banks.  Of a tile whose reduction runs down its rows,
-// [32 r][columns]: chunk c of row r at slot c ^ turn(r); a transposing read takes 4 rows x 32 bytes per 16 lanes, and those of 32
-// lanes (rows 8 apart) lie in all 64 banks.
-__device__ __forceinline__ int turn(int r) { return ((r & 3) << 2) | ((r >> 3 & 1) << 1); }
+// c ^ ((i >> 2) & 3), so that the chunks c of sixteen rows lie in all 64 banks.  Of a tile whose reduction runs down its rows: turn().
 
 // The operand of v_mfma_f32_16x16x32_bf16 out of such a tile: lane l gets column col + (l & 15), rows 8 (l >> 4) .. + 7.
 // ds_read_b64_tr_b16: lane i of 16 points at four neighbouring columns of a row (four lanes a row, four rows) and receives four rows
@@ -193,14 +192,6 @@ __device__ __forceinline__ bf16x8 tr_operand(const uint8_t *tile, int col, int l
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * ROW));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// The byte offsets, per lane, of kilobyte u of a [32 r][ROW / 2 columns] tile; columns behind the matrix read its last ones.
-template <int ROW>
-__device__ __forceinline__ uint32_t tr_offset(int u, int lane, long pitch, long last) {
-    constexpr int LANES = ROW / 16;
-    const int r = u * (64 / LANES) + lane / LANES, c = (lane % LANES) ^ turn(r);
-    return (uint32_t)r * (uint32_t)pitch + (uint32_t)min((long)c * 16, last);
 }
 
 // Tile of 64 IF x 32 JF, eight waves (4 x 2) of 16 IF x 16 JF, steps of 32 r.  Both operands come by LDS-DMA into rings of four parts (a
@@ -221,12 +212,12 @@ __device__ __forceinline__ void bw_product(const BwProduct &q, int bid, uint8_t 
 #pragma unroll
     for (int k = 0; k < NA; ++k) {
         const int u = wave + k * 8, row = u * 16 + (lane >> 2);
-        oa[k] = TRANS ? tr_offset<ROWA>(u, lane, q.pitch_a, q.pitch_a - 16 - i0 * 2L)
-                      : (uint32_t)min(row, q.I - 1 - i0) * (uint32_t)q.pitch_a + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
+        oa[k] = TRANS ? tr_offset<ROWA>(u, lane, q.a.pitch, q.a.width - i0 * 2L)
+                      : (uint32_t)min(row, q.I - 1 - i0) * (uint32_t)q.a.pitch + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
     }
 #pragma unroll
-    for (int k = 0; k < NB; ++k) ob[k] = tr_offset<ROWB>(wave + k * 8, lane, q.pitch_b, q.pitch_b - 16 - j0 * 2L);
-    const uint8_t *ab = q.a + (TRANS ? i0 * 2L : i0 * q.pitch_a), *bb = q.b + j0 * 2L;
+    for (int k = 0; k < NB; ++k) ob[k] = tr_offset<ROWB>(wave + k * 8, lane, q.pitch_b, q.pitch_b - j0 * 2L);
+    const uint8_t *ab = q.a.at + (TRANS ? i0 * 2L : i0 * q.a.pitch), *bb = q.b + j0 * 2L;
     // Load `k` of part t: its A's NA, then, where a step begins, B's NB.  Behind the end the last part is loaded again: the number of
     // loads in flight stays what the waits count.
     auto load = [&](int t, int k) {
@@ -234,7 +225,7 @@ __device__ __forceinline__ void bw_product(const BwProduct &q, int bid, uint8_t 
         t = min(t, parts - 1);
         const int s = t / P, p = t - s * P;
         if (k < NA)
-            dma16(ab + p * q.plane + (first + s) * (TRANS ? 32 * q.pitch_a : 64L), oa[k < NA ? k : 0], ta + slot * SA + (wave + k * 8) * 1024);
+            dma16(ab + p * q.a.plane + (first + s) * (TRANS ? 32 * q.a.pitch : 64L), oa[k < NA ? k : 0], ta + slot * SA + (wave + k * 8) * 1024);
         else
             dma16(bb + (first + s) * (32 * q.pitch_b), ob[k < NA ? 0 : k - NA], tb + slot_b * SB + (wave + (k - NA) * 8) * 1024);
     };
@@ -517,8 +508,7 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
     float *part = (float *)p;
     uint8_t *wx = p + pl.part, *ww = wx + pl.wx;
     float *px = (float *)(ww + pl.ww), *pw = (float *)((uint8_t *)px + pl.px);
-    // without a mask and with whole steps, bf16 gradients are their own single piece
-    const bool direct = type == PHONLP_BF16 && !bits && M % 32 == 0 && N % 32 == 0 && lddy % 8 == 0 && lddy < (1 << 22) && !((uintptr_t)dy & 15);
+    const bool direct = bw_direct(dy, type, lddy, bits, M, N);
     const bool make_planes = (dx || dw) && !direct;
     BwPrep prep = {dy, lddy, bits, make_planes ? (uint16_t *)planes : nullptr, !db ? nullptr : parts == 1 ? db : part,
                    {(const uint8_t *)x_codes, (const uint8_t *)w_codes}, {x_exponents, w_exponents}, {(__bf16 *)wx, (__bf16 *)ww}, {M, N},
@@ -530,12 +520,11 @@ extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, 
     };
     if (dw) prep.wide_blocks[0] = wide_blocks(M);
     if (dx) prep.wide_blocks[1] = wide_blocks(N);
-    const uint8_t *a = direct ? (const uint8_t *)dy : planes;
-    const long pitch = direct ? lddy * 2 : Np * 2L, plane = (long)Mp * Np * 2;
+    const BwOperand a = bw_dz(direct, dy, lddy, planes, N, Mp, Np);
     BwArgs g = {};
     const int TI = pl.IF * 64, TJ = pl.JF * 32;
-    g.x = {a, ww, nullptr, pitch, plane, Kp * 2L, M, K, N, ceil_div(M, TI), ceil_div(K, TJ), 0, 1, 0};
-    g.w = {a, wx, nullptr, pitch, plane, Kp * 2L, N, K, M, ceil_div(N, TI), ceil_div(K, TJ), 0, 1, 0};
+    g.x = {a, ww, nullptr, Kp * 2L, M, K, N, ceil_div(M, TI), ceil_div(K, TJ), 0, 1, 0};
+    g.w = {a, wx, nullptr, Kp * 2L, N, K, M, ceil_div(N, TI), ceil_div(K, TJ), 0, 1, 0};
     if (dx) set_split(g.x, pl.sx, dx, px);
     if (dw) set_split(g.w, pl.sw, dw, pw);
     g.part = part;
