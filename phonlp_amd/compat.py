@@ -395,25 +395,26 @@ def _loss_node(run, enc, params):
     return _HeadLossFn.apply(enc, run, names, *[params[k] for k in names])
 
 
-def parser_loss(heads, params, enc, sentlens, head, deprel, number_of_words=None, masks=None):
+def parser_loss(heads, params, enc, sentlens, head, deprel, number_of_words=None, masks=None, dense=None):
     """Differentiable `loss` of ref jointmodel/model.py:162-236 (dep_forward, eval=False, every dropout the identity) from the
     gathered encoder rows `enc` [B, L, E].  `params`: {reference parameter name: the live parameter} of the head modules
     (e.g. dict(model.named_parameters()) without the encoder's); `heads` must hold the same values (refresh_heads).
     loss.backward() then leaves in every parameter's .grad, and sends into `enc`, what the reference's own backward does.
-    `masks` (TaskHeads._parser_backward_train): the model in .train(), the dropout masks drawn by the caller."""
-    run = lambda e: (lambda o: {**o, "loss": o["loss"][4]})(heads.parser_backward(e, sentlens, head, deprel, number_of_words, masks))
+    `masks` (TaskHeads._parser_backward_train): the model in .train(), the dropout masks drawn by the caller.  `dense="e4m3"` (with masks)
+    runs this pass's large dense layers on 8-bit images, "f32" does not, None goes by the heads' cfg."""
+    run = lambda e: (lambda o: {**o, "loss": o["loss"][4]})(heads.parser_backward(e, sentlens, head, deprel, number_of_words, masks, dense))
     return _loss_node(run, enc, params)
 
 
-def pos_loss(heads, params, enc, sentlens, upos, ignore_index=1, masks=None):
-    """Differentiable `loss` of ref jointmodel/model.py:107-135 (pos_forward, use_soft_pos=False)."""
-    run = lambda e: (lambda o: {**o, "loss": o["loss"][0]})(heads.pos_backward(e, sentlens, upos, ignore_index, masks))
+def pos_loss(heads, params, enc, sentlens, upos, ignore_index=1, masks=None, dense=None):
+    """Differentiable `loss` of ref jointmodel/model.py:107-135 (pos_forward, use_soft_pos=False).  `masks`, `dense` as in parser_loss."""
+    run = lambda e: (lambda o: {**o, "loss": o["loss"][0]})(heads.pos_backward(e, sentlens, upos, ignore_index, masks, dense))
     return _loss_node(run, enc, params)
 
 
-def ner_loss(heads, params, enc, sentlens, tags, masks=None):
-    """Differentiable `loss` of ref jointmodel/model.py:139-160 (ner_forward: CRF NLL averaged over the batch)."""
-    return _loss_node(lambda e: heads.ner_backward(e, sentlens, tags, masks), enc, params)
+def ner_loss(heads, params, enc, sentlens, tags, masks=None, dense=None):
+    """Differentiable `loss` of ref jointmodel/model.py:139-160 (ner_forward: CRF NLL averaged over the batch).  `masks`, `dense` as in parser_loss."""
+    return _loss_node(lambda e: heads.ner_backward(e, sentlens, tags, masks, dense), enc, params)
 
 
 def _refuse_capture(name):
@@ -531,15 +532,14 @@ def _update(self, batch_dep=None, batch_pos=None, batch_ner=None, lambda_pos=1.0
     (draw_masks) and handed to the kernels' callers as inputs; the encoder trains as it is (its own dropout included)."""
     args = self.model.args
     p_drop, p_word = float(args.get("dropout", 0.0)), float(args.get("word_dropout", 0.0))
-    e4m3 = getattr(self, "_amd_dense", "f32") == "e4m3"
+    dense = getattr(self, "_amd_dense", "f32")
     self.model.train()
     h = refresh_heads(self.model)
-    h.cfg["e4m3_train"] = e4m3
     dev = h.w.trans.device
     params = {k: p for k, p in self.model.named_parameters() if not k.startswith("phobert.")}
     if "dep_hid.weight" not in params:  # a model that keeps its heads outside the module tree (tests/stub_model.py)
         params = {k: v for k, v in _head_state(self.model).items() if v.requires_grad}
-    train = p_drop > 0.0 or p_word > 0.0 or e4m3  # the 8-bit layers are those of the training-mode pass
+    train = p_drop > 0.0 or p_word > 0.0 or dense == "e4m3"  # the 8-bit layers are those of the training-mode pass
     if train and h.w.repl_dep is None:
         raise ValueError("phonlp_amd update(): word dropout and dense='e4m3' need the training model's drop_replacement_* parameters")
 
@@ -548,13 +548,13 @@ def _update(self, batch_dep=None, batch_pos=None, batch_ner=None, lambda_pos=1.0
 
     tok, fsw, _, head, rel, nwords, _, lens = batch_dep[:8]
     enc = _encode_train(self.model, tok, fsw)
-    l_dep = parser_loss(h, params, enc, lens, head, rel, nwords, masks("parser", enc, lens))
+    l_dep = parser_loss(h, params, enc, lens, head, rel, nwords, masks("parser", enc, lens), dense)
     tok, fsw, upos, _, lens = batch_pos[:5]
     enc = _encode_train(self.model, tok, fsw)
-    l_pos = pos_loss(h, params, enc, lens, upos, masks=masks("pos", enc, lens))
+    l_pos = pos_loss(h, params, enc, lens, upos, masks=masks("pos", enc, lens), dense=dense)
     tok, fsw, _, tags, _, lens = batch_ner[:6]
     enc = _encode_train(self.model, tok, fsw)
-    l_ner = ner_loss(h, params, enc, lens, tags, masks("ner", enc, lens))
+    l_ner = ner_loss(h, params, enc, lens, tags, masks("ner", enc, lens), dense)
     loss = lambda_pos * l_pos + lambda_ner * l_ner + lambda_dep * l_dep
     vals = (loss.item(), l_pos.item(), l_ner.item(), l_dep.item())
     loss.backward()

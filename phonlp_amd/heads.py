@@ -262,8 +262,8 @@ class TaskHeads:
             # engine 2, sentences of up to 512 words: the arc scorers' stages A and B in one kernel, fed by the image the
             # W1/W2 layer writes (0: stage A as a GEMM of its own, stage B converting fp32 operands: the round-2 form)
             "arc_fused": env("PHONLP_ARC_FUSED", "1") == "1",
-            # the training step's large dense layers (upos_hid, dep_hid, the scorers' first layers) on e4m3 images
-            # (patch_trainer(dense="e4m3")); the decoders and every eval-mode pass stay as they are
+            # a training pass's large dense layers (upos_hid, dep_hid, the scorers' first layers) on e4m3 images where the call
+            # does not say (`dense`); the decoders and every eval-mode pass stay as they are
             "e4m3_train": False,
         }
         self._side = None
@@ -348,16 +348,25 @@ class TaskHeads:
         return {"d_unlabeled": d_arc, "d_label": d_label, "d_lin": d_lin, "d_dist": d_dist}
 
     # ---- ... and on through the scorers and dep_hid: what loss.backward() leaves in the parameters' .grad
-    def parser_backward(self, enc: torch.Tensor, sentlens, gold_head, gold_rel, number_of_words=None, masks=None):
+    def _on_e4m3(self, dense, masks) -> bool:
+        """Whether this pass runs its large dense layers on 8-bit images: `dense` "f32" or "e4m3", None for the heads' own cfg."""
+        if dense not in (None, "f32", "e4m3"):
+            raise ValueError(f"dense must be 'f32' or 'e4m3', got {dense!r}")
+        if dense == "e4m3" and masks is None:
+            raise ValueError("dense='e4m3' is the training-mode pass's (masks)")
+        return self.cfg["e4m3_train"] if dense is None else dense == "e4m3"
+
+    def parser_backward(self, enc: torch.Tensor, sentlens, gold_head, gold_rel, number_of_words=None, masks=None, dense=None):
         """Backward of the parser loss (ref jointmodel/model.py:162-236, model in .eval()) through the four scorers and
         dep_hid -> {"grads": {reference parameter name: gradient in the reference's shape} for `unlabeled` / `deprel` /
         `linearization` / `distance` (.W1 / .W2 .weight, .bias, .scorer.W_bilin.weight), `dep_hid`, `upos_emb_matrix_dep`,
         `upos_hid`, `upos_clf`; "loss": fp32 [5] as parser_loss; "d_hidden": the gradient w.r.t. dep_hid's output [B,L,D]; "d_feat": w.r.t. its input
         [B,L,D] (= [enc ; pos_emb]; padded rows zero: the reference's padding is a constant); "d_enc": w.r.t. the
         gathered encoder rows [B,L,E], both routes added}.  Un-folded weights (the folds are an inference-time rewrite).
-        `masks`: the model in .train(), see _parser_backward_train."""
+        `masks`: the model in .train(), see _parser_backward_train; `dense="e4m3"`: its large dense layers on 8-bit images."""
+        e4m3 = self._on_e4m3(dense, masks)
         if masks is not None:
-            return self._parser_backward_train(enc, sentlens, gold_head, gold_rel, number_of_words, masks)
+            return self._parser_backward_train(enc, sentlens, gold_head, gold_rel, number_of_words, masks, e4m3)
         w = self.w
         n = w.n_arc_scorers
         dep = self.parser(enc, sentlens, want_raw=n > 1, want_label_argmax=False)
@@ -459,7 +468,7 @@ class TaskHeads:
             return d_xp * keep, d_embT.t().contiguous(), g
         return pos_emb, logits, backward
 
-    def _parser_backward_train(self, enc, sentlens, gold_head, gold_rel, number_of_words, masks):
+    def _parser_backward_train(self, enc, sentlens, gold_head, gold_rel, number_of_words, masks, e4m3):
         """dep_forward(eval=False) of the training model in .train() (ref jointmodel/model.py:162-236) and its backward, the
         random masks given by the caller in the padded layout: masks = {"wd_pos": bool [B,L] (word dropout in front of the
         POS layers), "drop_pos": [B,L,Hp] (nn.Dropout behind ReLU(upos_hid); kept entries carry 1/(1-p)), "wd": bool [B,L]
@@ -487,12 +496,12 @@ class TaskHeads:
         live = (torch.arange(L, device=dev)[None, :] < lens[:, None]).reshape(M, 1)
         x = enc.reshape(M, E).contiguous()
         pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_dep, bl(masks["wd_pos"]), f32(masks["drop_pos"]).reshape(M, -1),
-                                                       self.cfg["e4m3_train"])
+                                                       e4m3)
         feat = torch.cat([x, pos_emb], 1).contiguous()
         m_wd = bl(masks["wd"])
         featd = TaskHeads._word_drop(feat, m_wd, w.repl_dep)
         # dep_hid; the padded rows of its output are the zeros of pad_packed_sequence (:182-183)
-        hidden, hidden_bw = _dense(featd, w.dep_hid_w, w.dep_hid_b, False, self.cfg["e4m3_train"])
+        hidden, hidden_bw = _dense(featd, w.dep_hid_w, w.dep_hid_b, False, e4m3)
         hidden = (hidden * live).contiguous()
 
         def first_layer(name, W12, b12, row0):
@@ -505,7 +514,7 @@ class TaskHeads:
                 Wk, bk = W12[row0 + k * KP:row0 + (k + 1) * KP].contiguous(), b12[row0 + k * KP:row0 + (k + 1) * KP].contiguous()
                 mk = torch.ones((M, KP), dtype=torch.float32, device=dev)  # the ones column (appended behind the dropout) stays
                 mk[:, :H] = f32(ms[k]).reshape(M, H)
-                if self.cfg["e4m3_train"]:
+                if e4m3:
                     y, layer_bw = _dense(hin, Wk, bk, True, True)
                     y = (y * mk).contiguous()
                 else:  # the masked output carries the ReLU's mask: dropped entries get no gradient either way
@@ -593,12 +602,14 @@ class TaskHeads:
                                               "upos_clf.bias": dbc}
 
     # ---- the NER loss's backward (ref jointmodel/model.py:139-160 + crf.py:24-46 under loss.backward(), model in .eval())
-    def ner_backward(self, enc: torch.Tensor, sentlens, gold_tags, masks=None):
+    def ner_backward(self, enc: torch.Tensor, sentlens, gold_tags, masks=None, dense=None):
         """-> {"loss": the batch-averaged CRF NLL (0-dim), "grads": {"ner_tag_clf.weight", "ner_tag_clf.bias", "crit_ner._transitions", "upos_emb_matrix_ner",
         "upos_hid.*", "upos_clf.*"}, "d_enc": the gradient w.r.t. the gathered encoder rows [B,L,E]}: CRF NLL averaged
         over the batch -> ReLU -> ner_tag_clf -> [enc ; soft POS embedding] -> the POS layers.  `masks` (model in .train()):
-        {"wd_pos", "drop_pos"} as in _parser_backward_train and "wd": bool [B,L], the word dropout on [enc ; pos_emb] (:155)."""
+        {"wd_pos", "drop_pos"} as in _parser_backward_train and "wd": bool [B,L], the word dropout on [enc ; pos_emb] (:155).
+        `dense` as in parser_backward."""
         w = self.w
+        e4m3 = self._on_e4m3(dense, masks)
         if masks is not None:
             lens = as_sentlens(sentlens, enc.device)
             B, L, E = enc.shape
@@ -608,7 +619,7 @@ class TaskHeads:
             x = enc.reshape(M, E).contiguous()
             pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_ner, bl(masks["wd_pos"]),
                                                            torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1),
-                                                           self.cfg["e4m3_train"])
+                                                           e4m3)
             m_wd = bl(masks["wd"])
             featd = TaskHeads._word_drop(torch.cat([x, pos_emb], 1).contiguous(), m_wd, w.repl_ner)
             logits2 = (ops.linear(featd, w.ner_w, w.ner_b, True, None, 0) * live).contiguous()
@@ -643,10 +654,12 @@ class TaskHeads:
         return {"loss": loss, "grads": grads, "d_enc": (d_feat[:, :E] + d_x).view(B, L, E)}
 
     # ---- ... and its backward through upos_clf and upos_hid (what loss.backward() leaves behind pos_forward)
-    def pos_backward(self, enc: torch.Tensor, sentlens, gold_upos, ignore_index=1, masks=None):
+    def pos_backward(self, enc: torch.Tensor, sentlens, gold_upos, ignore_index=1, masks=None, dense=None):
         """-> {"loss": fp32 [3] as pos_loss, "grads": {"upos_hid.weight", "upos_hid.bias", "upos_clf.weight",
-        "upos_clf.bias"}, "d_enc": the gradient w.r.t. the gathered encoder rows [B,L,E] (zero on padding)}."""
+        "upos_clf.bias"}, "d_enc": the gradient w.r.t. the gathered encoder rows [B,L,E] (zero on padding)}.  `dense` as in
+        parser_backward."""
         w = self.w
+        e4m3 = self._on_e4m3(dense, masks)
         lens = as_sentlens(sentlens, enc.device)
         B, L, E = enc.shape
         M = B * L
@@ -656,7 +669,7 @@ class TaskHeads:
             m_wd = torch.as_tensor(masks["wd_pos"]).to(device=dev, dtype=torch.bool).reshape(M)
             m_dp = torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1)
             xp = TaskHeads._word_drop(x, m_wd, w.repl_pos)
-            hid, hid_bw = _dense(xp, w.upos_hid_w, w.upos_hid_b, True, self.cfg["e4m3_train"])
+            hid, hid_bw = _dense(xp, w.upos_hid_w, w.upos_hid_b, True, e4m3)
             hid_d = (hid * m_dp).contiguous()
             logits = ops.linear(hid_d, w.upos_clf_w, w.upos_clf_b, False, None, 0).view(B, L, -1)
             gold = torch.as_tensor(gold_upos).to(device=dev, dtype=torch.int32).contiguous()
