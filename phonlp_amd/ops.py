@@ -968,8 +968,8 @@ _PLAIN = {Tensor, torch.nn.Parameter}
 
 
 def _traced(t: Tensor) -> bool:
-    """A fake tensor, or a call that torch.compile traces: it goes through the registered op (below), which an eager call leaves out for
-    its host time."""
+    """A fake tensor or another subclass, or a call that torch.compile traces: it goes through the registered op (below), whose body is
+    the `_now` function; an eager call on plain tensors takes that at once, for its host time."""
     return type(t) not in _PLAIN or torch.compiler.is_compiling()
 
 
@@ -1035,8 +1035,10 @@ def e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
     """x [rows, K] fp32 / bf16 / fp16 (row stride free, unit column stride) -> its e4m3 image: codes float8_e4m3fn
     [rows, e4m3_kp(K)], exponents uint8 [rows, e4m3_kb(K)] (one power-of-two scale per row and block of 128 columns; infinities and
     NaN become NaN).  The operand form of linear_e4m3, and a layer input's 8-bit checkpoint for linear_e4m3_backward."""
-    if _traced(x):
-        return torch.ops.phonlp_amd.e4m3_rows(x)
+    return torch.ops.phonlp_amd.e4m3_rows(x) if _traced(x) else _e4m3_rows_now(x)
+
+
+def _e4m3_rows_now(x: Tensor) -> Tuple[Tensor, Tensor]:
     code, ld, rows, K = _rows_of(x, "x")
     if K == 0:
         raise ValueError("e4m3_rows: x has no columns")
@@ -1050,8 +1052,10 @@ def e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
 
 def e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype = torch.float32) -> Tensor:
     """The values [rows, K] that an e4m3 image stands for: exact in fp32 and bf16, 16-bit types saturate at their largest."""
-    if _traced(codes):
-        return torch.ops.phonlp_amd.e4m3_values(codes, exponents, K, dtype)
+    return (torch.ops.phonlp_amd.e4m3_values if _traced(codes) else _e4m3_values_now)(codes, exponents, K, dtype)
+
+
+def _e4m3_values_now(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype) -> Tensor:
     rows = _image_of(codes, exponents, K, "codes")
     if dtype not in _TYPES:
         raise ValueError(f"e4m3_values: dtype must be float32, bfloat16 or float16, got {dtype}")
@@ -1070,6 +1074,10 @@ def linear_e4m3(x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponen
     if _traced(x_codes):
         y, bits = torch.ops.phonlp_amd.linear_e4m3(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits)
         return y, bits if want_bits else None
+    return _linear_e4m3_now(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits)
+
+
+def _linear_e4m3_now(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits) -> Tuple[Tensor, Optional[Tensor]]:
     M = _image_of(x_codes, x_exponents, K, "x_codes")
     N = _image_of(w_codes, w_exponents, K, "w_codes")
     dev = x_codes.device
@@ -1130,8 +1138,10 @@ def _tokens_of(tokens: Tensor, device) -> int:
 def embedding_rows(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
     """scale * table[tokens]: table [V, E] fp32 / bf16 / fp16 (row stride free), tokens int32 / int64 of any shape -> [*tokens.shape,
     E] of the table's type.  A token outside [0, V) gives a row of zeros."""
-    if _traced(table):
-        return torch.ops.phonlp_amd.embedding_rows(table, tokens, scale)
+    return (torch.ops.phonlp_amd.embedding_rows if _traced(table) else _embedding_rows_now)(table, tokens, scale)
+
+
+def _embedding_rows_now(table: Tensor, tokens: Tensor, scale: float) -> Tensor:
     code, ld, V, E = _rows_of(table, "table")
     N = _tokens_of(tokens, table.device)
     out = torch.empty((*tokens.shape, E), dtype=table.dtype, device=table.device)
@@ -1175,7 +1185,7 @@ def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.
 # The forward ones as registered ops, for tracing; without bits linear_e4m3 returns an empty tensor in their place.
 @torch.library.custom_op("phonlp_amd::e4m3_rows", mutates_args=())
 def _e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
-    return e4m3_rows(x)
+    return _e4m3_rows_now(x)
 
 
 @_e4m3_rows.register_fake
@@ -1186,7 +1196,7 @@ def _(x):
 
 @torch.library.custom_op("phonlp_amd::e4m3_values", mutates_args=())
 def _e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype) -> Tensor:
-    return e4m3_values(codes, exponents, K, dtype)
+    return _e4m3_values_now(codes, exponents, K, dtype)
 
 
 @_e4m3_values.register_fake
@@ -1197,7 +1207,7 @@ def _(codes, exponents, K, dtype):
 @torch.library.custom_op("phonlp_amd::linear_e4m3", mutates_args=())
 def _linear_e4m3(x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponents: Tensor, bias: Optional[Tensor], K: int, relu: bool,
                  dtype: torch.dtype, want_bits: bool) -> Tuple[Tensor, Tensor]:
-    y, bits = linear_e4m3(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits)
+    y, bits = _linear_e4m3_now(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bits)
     return y, y.new_empty((0,), dtype=torch.int32) if bits is None else bits
 
 
@@ -1210,7 +1220,7 @@ def _(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bit
 
 @torch.library.custom_op("phonlp_amd::embedding_rows", mutates_args=())
 def _embedding_rows(table: Tensor, tokens: Tensor, scale: float) -> Tensor:
-    return embedding_rows(table, tokens, scale)
+    return _embedding_rows_now(table, tokens, scale)
 
 
 @_embedding_rows.register_fake
