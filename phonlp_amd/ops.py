@@ -1100,6 +1100,13 @@ def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_
     """Backward of linear_e4m3 from the checkpoint: dY [M, N] fp32 / bf16 / fp16 (row stride free), bits of a ReLU layer (None: no
     ReLU), the images of the layer's input and weight -> (dX [M, K] of dY's type, dW [N, K] fp32, db [N] fp32), None where not asked
     for.  The quantisation of x and w counts as the identity."""
+    if _traced(dY):
+        got = torch.ops.phonlp_amd.linear_e4m3_backward(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db)
+        return tuple(t if on else None for t, on in zip(got, (need_dX, need_dW, need_db)))
+    return _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db)
+
+
+def _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db):
     code, ld, *shape = _rows_of(dY, "dY")
     M = _image_of(x_codes, x_exponents, K, "x_codes")
     N = _image_of(w_codes, w_exponents, K, "w_codes")
@@ -1157,6 +1164,10 @@ def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.
     """Gradient of embedding_rows for its table: d_out [*tokens.shape, E] -> d_table [V, E], d_table[v] = scale * the sum of the rows
     whose token is v (zeros where there are none), of d_out's type or `dtype` = float32.  Sums in fp32, by sorted tokens: the same
     tokens give the same bits."""
+    return (torch.ops.phonlp_amd.embedding_rows_grad if _traced(d_out) else _embedding_rows_grad_now)(d_out, tokens, V, scale, dtype)
+
+
+def _embedding_rows_grad_now(d_out: Tensor, tokens: Tensor, V: int, scale: float, dtype: Optional[torch.dtype]) -> Tensor:
     if d_out.dim() < 1 or tuple(d_out.shape[:-1]) != tuple(tokens.shape):
         raise ValueError(f"d_out: expected [*{tuple(tokens.shape)}, E], got {tuple(d_out.shape)}")
     E = d_out.shape[-1]
@@ -1182,7 +1193,7 @@ def embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float = 1.
     return d_table
 
 
-# The forward ones as registered ops, for tracing; without bits linear_e4m3 returns an empty tensor in their place.
+# As registered ops, for tracing; bits and gradients that are not asked for are empty tensors there.
 @torch.library.custom_op("phonlp_amd::e4m3_rows", mutates_args=())
 def _e4m3_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
     return _e4m3_rows_now(x)
@@ -1218,6 +1229,21 @@ def _(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bit
             x_codes.new_empty((M, (N + 31) // 32) if want_bits else (0,), dtype=torch.int32))
 
 
+@torch.library.custom_op("phonlp_amd::linear_e4m3_backward", mutates_args=())
+def _linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponents: Tensor,
+                          K: int, need_dX: bool, need_dW: bool, need_db: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    got = _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db)
+    types = dY.dtype, torch.float32, torch.float32
+    return tuple(dY.new_empty((0,), dtype=t) if g is None else g for g, t in zip(got, types))
+
+
+@_linear_e4m3_backward.register_fake
+def _(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db):
+    M, N = x_codes.shape[0], w_codes.shape[0]
+    return (dY.new_empty((M, K) if need_dX else (0,)), dY.new_empty((N, K) if need_dW else (0,), dtype=torch.float32),
+            dY.new_empty((N,) if need_db else (0,), dtype=torch.float32))
+
+
 @torch.library.custom_op("phonlp_amd::embedding_rows", mutates_args=())
 def _embedding_rows(table: Tensor, tokens: Tensor, scale: float) -> Tensor:
     return _embedding_rows_now(table, tokens, scale)
@@ -1226,6 +1252,16 @@ def _embedding_rows(table: Tensor, tokens: Tensor, scale: float) -> Tensor:
 @_embedding_rows.register_fake
 def _(table, tokens, scale):
     return table.new_empty((*tokens.shape, table.shape[1]))
+
+
+@torch.library.custom_op("phonlp_amd::embedding_rows_grad", mutates_args=())
+def _embedding_rows_grad(d_out: Tensor, tokens: Tensor, V: int, scale: float, dtype: Optional[torch.dtype]) -> Tensor:
+    return _embedding_rows_grad_now(d_out, tokens, V, scale, dtype)
+
+
+@_embedding_rows_grad.register_fake
+def _(d_out, tokens, V, scale, dtype):
+    return d_out.new_empty((V, d_out.shape[-1]), dtype=dtype)
 
 
 # ---- shape functions (torch.library `register_fake`) for the ops above that had none: with them every custom op of

@@ -18,3 +18,27 @@ def test_subclasses_meet_the_arguments_own_checks():
                         ("table: expected a ROCm", lambda: ops.embedding_rows(x, tokens))):
         with pytest.raises(ValueError, match=match):
             call()
+
+
+def _fake_operands():
+    x, w = torch.empty(28, 200, dtype=torch.bfloat16, device="cuda"), torch.empty(33, 200, device="cuda")
+    return x, w, ops.e4m3_rows(x), ops.e4m3_rows(w)
+
+
+def test_the_gradients_trace_on_fake_tensors():
+    """Shapes and types flow through both gradients, each output asked for or not."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, w, xi, wi = _fake_operands()
+        dY, bits = torch.empty(28, 33, dtype=torch.float16, device="cuda"), torch.empty(28, 2, dtype=torch.int32, device="cuda")
+        dX, dW, db = ops.linear_e4m3_backward(dY, bits, *xi, *wi, 200)
+        assert dX.shape == (28, 200) and dX.dtype == torch.float16 and dX.is_cuda
+        assert dW.shape == (33, 200) and db.shape == (33,) and dW.dtype == db.dtype == torch.float32
+        dX, dW, db = ops.linear_e4m3_backward(dY, None, *xi, *wi, 200, False, True, False)
+        assert dX is None and db is None and dW.shape == (33, 200)
+        tokens = torch.empty(4, 7, dtype=torch.int32, device="cuda")
+        d = torch.empty(4, 7, 100, dtype=torch.bfloat16, device="cuda")
+        for dtype in (None, torch.bfloat16, torch.float32):
+            g = ops.embedding_rows_grad(d, tokens, 50, 2.0, dtype)
+            assert g.shape == (50, 100) and g.dtype == (dtype or torch.bfloat16) and g.is_cuda
