@@ -236,7 +236,7 @@ struct SumArgs {
     void *d_table;
     float *shares;  // [chunks][2][E]: the sum of a chunk's first run that began before it, of its last run that goes on behind it
     const int *order, *sorted;
-    long ld;
+    long ld, row0;  // row0: the table's first row of this launch
     int N, V, E, R, chunks, sum_blocks;
     float scale;
 };
@@ -248,14 +248,15 @@ struct SumArgs {
 // fp32, 512 tokens 4.2 against 13.5; at worst, 512 times the same token of 1000 x 768 bf16, 30 against 15.
 constexpr int kFewMost = 512;
 template <int VEC, class T, class TO, class I>
-__global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld, const I *tokens, int N, int V, int E, int rows, float scale, TO *table) {
+__global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld, const I *tokens, int N, int V, int E, long base, int rows, float scale,
+                                                            TO *table) {
     constexpr int UNROLL = 16;
     typedef typename Vec<T, VEC>::type Vt;
     __shared__ float shares[4][64 * VEC];
     __shared__ unsigned there[4][2];  // of each wave, the rows that it has tokens of
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = (blockIdx.y * 64 + lane) * VEC,
               col = min(from, E - VEC), each = ceil_div(N, 4), first = wave * each, mine = min(each, N - first);
-    const long row0 = (long)blockIdx.x * rows;
+    const long row0 = base + (long)blockIdx.x * rows;
     const int have = (int)min((long)rows, V - row0);
     if (threadIdx.x < 8) there[threadIdx.x >> 1][threadIdx.x & 1] = 0;
     __syncthreads();
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(SumArgs a) {
     TO *table = (TO *)a.d_table;
     if ((int)blockIdx.x >= a.sum_blocks) {
         if (blockIdx.y) return;
-        const long row0 = ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 16;
+        const long row0 = a.row0 + ((long)(blockIdx.x - a.sum_blocks) * 4 + wave) * 16;
         if (row0 >= a.V) return;
         unsigned long long rows = (1ull << min(a.V - row0, 16L)) - 1;  // those that no token points at
         const int from = lower_bound_wave(a.sorted, a.N, (int)row0, lane);
@@ -467,6 +468,8 @@ __global__ __launch_bounds__(512) void embedding_join_kernel(SumArgs a) {
     }
 }
 
+// Tokens or rows of the table that one launch covers: a grid holds less than 2^32 threads.
+constexpr int kLaunchMost = 1 << 29;
 constexpr int kPlaceMost = 8192;  // tokens sorted by counting (above)
 struct EmbeddingPlan {
     int R, chunks, tile, tiles;  // places of one wave; pairs of a sorting tile
@@ -520,10 +523,15 @@ static int sum_rows(SumArgs a, hipStream_t st) {
     a.sum_blocks = ceil_div(a.chunks, 4);
     {
         ProfScope ps("embedding_sum", st);
-        hipLaunchKernelGGL((embedding_sum_kernel<VEC, T, TO>), dim3(a.sum_blocks + ceil_div(a.V, 64), slabs), dim3(256), 0, st, a);
-        const int rc = check_launch("embedding_sum_kernel");
-        if (rc || a.chunks == 1) return rc;
+        do {
+            const int rows = (int)(a.V - a.row0 < kLaunchMost ? a.V - a.row0 : kLaunchMost);
+            hipLaunchKernelGGL((embedding_sum_kernel<VEC, T, TO>), dim3(a.sum_blocks + ceil_div(rows, 64), slabs), dim3(256), 0, st, a);
+            const int rc = check_launch("embedding_sum_kernel");
+            if (rc) return rc;
+            a.sum_blocks = 0;  // the sums are made
+        } while ((a.row0 += kLaunchMost) < a.V);
     }
+    if (a.chunks == 1) return PHONLP_OK;
     ProfScope ps("embedding_join", st);
     hipLaunchKernelGGL((embedding_join_kernel<VEC, TO>), dim3(ceil_div(a.chunks - 1, 8), slabs), dim3(512), 0, st, a);
     return check_launch("embedding_join_kernel");
@@ -533,9 +541,14 @@ template <int VEC, class T, class TO, class I>
 static int few_rows(const SumArgs &a, const I *tokens, hipStream_t st) {
     ProfScope ps("embedding_few", st);
     const int rows = a.V >= 65536 ? 64 : ceil_div(a.V, 1024);  // of a workgroup: some thousand of them a slab
-    hipLaunchKernelGGL((embedding_few_kernel<VEC, T, TO, I>), dim3(ceil_div(a.V, rows), ceil_div(a.E, 64 * VEC)), dim3(256), 0,
-                       st, (const T *)a.d_out, a.ld, tokens, a.N, a.V, a.E, rows, a.scale, (TO *)a.d_table);
-    return check_launch("embedding_few_kernel");
+    for (long base = 0; base < a.V; base += kLaunchMost) {
+        const int most = (int)(a.V - base < kLaunchMost ? a.V - base : kLaunchMost);
+        hipLaunchKernelGGL((embedding_few_kernel<VEC, T, TO, I>), dim3(ceil_div(most, rows), ceil_div(a.E, 64 * VEC)), dim3(256), 0, st,
+                           (const T *)a.d_out, a.ld, tokens, a.N, a.V, a.E, base, rows, a.scale, (TO *)a.d_table);
+        const int rc = check_launch("embedding_few_kernel");
+        if (rc) return rc;
+    }
+    return PHONLP_OK;
 }
 
 // Calls f with the widest vector of T (16 bytes, 4 elements or one) that a row of E holds.
@@ -563,14 +576,18 @@ extern "C" int phonlp_embedding_rows(const void *table, int type, long ld, const
         using T = decltype(t);
         return with_vec<T>(E, [&](auto vec) {
             constexpr int VEC = decltype(vec)::value;
-            const dim3 grid(ceil_div(ceil_div(N, 16), 4), ceil_div(E, 64 * VEC));
-            if (tokens_are_int64)
-                hipLaunchKernelGGL((embedding_rows_kernel<VEC, T, long>), grid, dim3(256), 0, st, (const T *)table, ld, (const long *)tokens, N,
-                                   V, E, scale, (T *)out);
-            else
-                hipLaunchKernelGGL((embedding_rows_kernel<VEC, T, int>), grid, dim3(256), 0, st, (const T *)table, ld, (const int *)tokens, N,
-                                   V, E, scale, (T *)out);
-            return check_launch("embedding_rows_kernel");
+            auto launch = [&](auto *tok) {
+                using I = std::remove_cv_t<std::remove_pointer_t<decltype(tok)>>;
+                for (long n = 0; n < N; n += kLaunchMost) {
+                    const int most = (int)(N - n < kLaunchMost ? N - n : kLaunchMost);
+                    hipLaunchKernelGGL((embedding_rows_kernel<VEC, T, I>), dim3(ceil_div(most, 64), ceil_div(E, 64 * VEC)), dim3(256), 0, st,
+                                       (const T *)table, ld, tok + n, most, V, E, scale, (T *)out + n * E);
+                    const int rc = check_launch("embedding_rows_kernel");
+                    if (rc) return rc;
+                }
+                return (int)PHONLP_OK;
+            };
+            return tokens_are_int64 ? launch((const long *)tokens) : launch((const int *)tokens);
         });
     });
 }
@@ -590,7 +607,7 @@ extern "C" int phonlp_embedding_rows_grad(const void *d_out, int type, long ld, 
         return fail(PHONLP_ERR_WORKSPACE, "embedding_rows_grad: workspace too small or not 16-byte aligned");
     hipStream_t st = as_stream(stream);
     const EmbeddingPlan pl = plan_embedding(N, E);
-    SumArgs a = {d_out, d_table, nullptr, nullptr, nullptr, ld, N, V, E, pl.R, pl.chunks, 0, scale};
+    SumArgs a = {d_out, d_table, nullptr, nullptr, nullptr, ld, 0, N, V, E, pl.R, pl.chunks, 0, scale};
     const bool few = N <= kFewMost, radix = N > kPlaceMost;
     if (!few) {
         int *order, *sorted;

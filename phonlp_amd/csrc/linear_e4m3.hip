@@ -384,7 +384,8 @@ extern "C" int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponent
     if (((uintptr_t)x_codes & 15) || ((uintptr_t)w_codes & 15) || ((uintptr_t)x_exponents & 3) || ((uintptr_t)w_exponents & 3) ||
         ((uintptr_t)bias & 3) || ((uintptr_t)bits & 3) || (uintptr_t)y % type_bytes(type))
         return fail(PHONLP_ERR_SHAPE, "linear_e4m3: codes must be 16-byte aligned, exponents, bias and bits 4-byte, y to its type");
-    if ((long)ceil_div(M, 32) * ceil_div(N, 32) > 0x3FFFFFFF) return fail(PHONLP_ERR_UNSUPPORTED, "linear_e4m3: M * N too large");
+    // a grid holds less than 2^32 threads
+    if ((M + 127L) / 128 * ((N + 127L) / 128) >= 1 << 23) return fail(PHONLP_ERR_UNSUPPORTED, "linear_e4m3: M * N too large");
     E4m3Args a = {(const uint8_t *)x_codes, x_exponents, (const uint8_t *)w_codes, w_exponents, bias, y, (uint8_t *)bits, M, N, kp8_of(K),
                   kb4_of(K), 0, 0, relu, ceil_div(N, 32) * 4};
     hipStream_t st = as_stream(stream);

@@ -482,7 +482,7 @@ using namespace phonlp;
 
 static bool bw_shape_ok(int M, int N, int K, int type) {
     return M > 0 && N > 0 && K > 0 && K <= (1 << 21) && N <= (1 << 21) && M <= (1 << 24) && type_ok(type) &&
-           (long)ceil_div(M, 128) * ceil_div(K, 128) < (1L << 24) && (long)ceil_div(N, 128) * ceil_div(K, 128) < (1L << 24);
+           (long)ceil_div(M, 128) * ceil_div(K, 128) < (1L << 22) && (long)ceil_div(N, 128) * ceil_div(K, 128) < (1L << 22);
 }
 
 extern "C" size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int type) {
