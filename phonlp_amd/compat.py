@@ -481,6 +481,8 @@ def linear_e4m3(x, weight, bias=None, relu=False):
     """Differentiable y = act(x @ weight.T + bias) with both operands in e4m3 (a power-of-two scale per row and block of 128 columns),
     fp32 sums, y of x's type: x [..., K], weight [N, K], bias [N] in fp32 / bf16 / fp16.  What it keeps for the backward is the 8-bit
     images and one bit per output of a ReLU; the quantisation counts as the identity.  Under torch.no_grad nothing is kept."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:  # an image does not know where inside its last block K ends
+        raise ValueError(f"weight: expected [N, K] with x's K columns, got {tuple(weight.shape)} for x {tuple(x.shape)}")
     return _LinearE4m3Fn.apply(x, weight, bias, bool(relu))
 
 
