@@ -496,10 +496,12 @@ def _encode_train(model, tokens, first_subword):
     if emb.is_cuda and emb.dtype in (torch.float32, torch.bfloat16, torch.float16):
         B, S, E = emb.shape
         first = first_subword.long()
+        if first.dim() != 2 or first.shape[0] > B:
+            raise ValueError(f"first_subword: expected at most {B} rows of indices, got {tuple(first.shape)}")
         if not first.is_cuda and first.numel() and not 0 <= int(first.min()) <= int(first.max()) < S:
             raise IndexError(f"first_subword: expected indices below {S}, got {int(first.min())} to {int(first.max())}")
         first = first.to(enc_dev)
-        rows = torch.where((first >= 0) & (first < S), first + torch.arange(B, device=enc_dev)[:, None] * S, -1)
+        rows = torch.where((first >= 0) & (first < S), first + torch.arange(first.shape[0], device=enc_dev)[:, None] * S, -1)
         return embedding_rows(emb.reshape(B * S, E).contiguous(), rows).float().to(dev)
     idx = first_subword.to(enc_dev).long().unsqueeze(-1).expand(-1, -1, emb.shape[-1])
     return torch.gather(emb, 1, idx).float().to(dev)
