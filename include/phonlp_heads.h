@@ -535,8 +535,9 @@ int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponents, const vo
 
 /* Backward of that layer from its 8-bit checkpoint: dY [M,N] in `type` (row pitch lddy), bits as above (NULL: no ReLU), the images
  * of the layer's input and weight ->  dZ = dY where the bit is set, dX [M,K] = dZ . W^ in `type`, dW [N,K] = dZ^T . X^ and
- * db [N] = column sums of dZ in fp32.  Any of dX / dW / db may be NULL.  Products are exact (dZ in up to three bf16 pieces), sums
- * fp32 in a fixed order.  M <= 2^24, N and K <= 2^21, ceil(M / 128) * ceil(K / 128) and ceil(N / 128) * ceil(K / 128) < 2^22. */
+ * db [N] = column sums of dZ in fp32.  Any of dX / dW / db may be NULL, x's image without dW and w's without dX too.  Products are
+ * exact (dZ in up to three bf16 pieces), sums fp32 in a fixed order.  M <= 2^24, N and K <= 2^21; ceil(M / 128) * ceil(K / 128) and
+ * ceil(N / 128) * ceil(K / 128) < 2^22. */
 size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int type);
 int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, const uint32_t *bits, const void *x_codes,
                                 const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents, int M, int N, int K,

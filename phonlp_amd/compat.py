@@ -460,7 +460,8 @@ class _LinearE4m3Fn(torch.autograd.Function):
         xi, wi = ops.e4m3_rows(x.reshape(x.shape[:-1].numel(), K).contiguous()), ops.e4m3_rows(weight.contiguous())
         y, bits = ops.linear_e4m3(*xi, *wi, None if bias is None else bias.float().contiguous(), K, relu, x.dtype,
                                   relu and any(ctx.needs_input_grad))
-        ctx.save_for_backward(*xi, *wi, bits)
+        need_x, need_w, *_ = ctx.needs_input_grad  # x's image is dW's operand, w's is dX's
+        ctx.save_for_backward(*(xi if need_w else (None, None)), *(wi if need_x else (None, None)), bits)
         ctx.K, ctx.shape = K, x.shape
         ctx.types = weight.dtype, None if bias is None else bias.dtype
         return y.view(*x.shape[:-1], weight.shape[0])
@@ -471,16 +472,15 @@ class _LinearE4m3Fn(torch.autograd.Function):
         _refuse_capture("linear_e4m3")
         *images, bits = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dX, dW, db = ops.linear_e4m3_backward(g.reshape(images[0].shape[0], images[2].shape[0]).contiguous(), bits, *images, ctx.K,
-                                              *need[:3])
+        dX, dW, db = ops.linear_e4m3_backward(g.reshape(ctx.shape[:-1].numel(), g.shape[-1]).contiguous(), bits, *images, ctx.K, *need[:3])
         return (None if dX is None else dX.view(ctx.shape), None if dW is None else dW.to(ctx.types[0]),
                 None if db is None else db.to(ctx.types[1]), None)
 
 
 def linear_e4m3(x, weight, bias=None, relu=False):
     """Differentiable y = act(x @ weight.T + bias) with both operands in e4m3 (a power-of-two scale per row and block of 128 columns),
-    fp32 sums, y of x's type: x [..., K], weight [N, K], bias [N] in fp32 / bf16 / fp16.  What it keeps for the backward is the 8-bit
-    images and one bit per output of a ReLU; the quantisation counts as the identity.  Under torch.no_grad nothing is kept."""
+    fp32 sums, y of x's type: x [..., K], weight [N, K], bias [N] in fp32 / bf16 / fp16.  What it keeps for the backward are the 8-bit
+    images (x's where weight, weight's where x needs a gradient) and one bit per output of a ReLU; the quantisation counts as the identity.  Under torch.no_grad nothing is kept."""
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:  # an image does not know where inside its last block K ends
         raise ValueError(f"weight: expected [N, K] with x's K columns, got {tuple(weight.shape)} for x {tuple(x.shape)}")
     return _LinearE4m3Fn.apply(x, weight, bias, bool(relu))

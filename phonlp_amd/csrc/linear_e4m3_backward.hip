@@ -492,7 +492,7 @@ extern "C" size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int 
 extern "C" int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, const uint32_t *bits, const void *x_codes,
                                            const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents, int M, int N, int K,
                                            void *dx, float *dw, float *db, void *ws, size_t ws_bytes, void *stream) {
-    if (!dy || !x_codes || !x_exponents || !w_codes || !w_exponents || !bw_shape_ok(M, N, K, type) || lddy < N)
+    if (!dy || (dw && (!x_codes || !x_exponents)) || (dx && (!w_codes || !w_exponents)) || !bw_shape_ok(M, N, K, type) || lddy < N)
         return fail(PHONLP_ERR_SHAPE, "linear_e4m3_backward: bad argument");
     if (((uintptr_t)x_codes & 15) || ((uintptr_t)w_codes & 15) || ((uintptr_t)x_exponents & 3) || ((uintptr_t)w_exponents & 3) ||
         ((uintptr_t)bits & 3) || ((uintptr_t)dw & 3) || ((uintptr_t)db & 3) || (uintptr_t)dy % type_bytes(type) ||

@@ -1095,11 +1095,13 @@ def _linear_e4m3_now(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, 
     return y, bits
 
 
-def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor,
-                         w_exponents: Tensor, K: int, need_dX: bool = True, need_dW: bool = True, need_db: bool = True):
+def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Optional[Tensor], x_exponents: Optional[Tensor],
+                         w_codes: Optional[Tensor], w_exponents: Optional[Tensor], K: int, need_dX: bool = True, need_dW: bool = True,
+                         need_db: bool = True):
     """Backward of linear_e4m3 from the checkpoint: dY [M, N] fp32 / bf16 / fp16 (row stride free), bits of a ReLU layer (None: no
     ReLU), the images of the layer's input and weight -> (dX [M, K] of dY's type, dW [N, K] fp32, db [N] fp32), None where not asked
-    for.  The quantisation of x and w counts as the identity."""
+    for.  The quantisation of x and w counts as the identity.  x's image is dW's operand and w's is dX's: each may be None where that
+    is not asked for."""
     if _traced(dY):
         got = torch.ops.phonlp_amd.linear_e4m3_backward(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db)
         return tuple(t if on else None for t, on in zip(got, (need_dX, need_dW, need_db)))
@@ -1108,8 +1110,17 @@ def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_
 
 def _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db):
     code, ld, *shape = _rows_of(dY, "dY")
-    M = _image_of(x_codes, x_exponents, K, "x_codes")
-    N = _image_of(w_codes, w_exponents, K, "w_codes")
+    M, N = shape
+    for codes, exponents, need, name, of in ((x_codes, x_exponents, need_dW, "x_codes", "dW"), (w_codes, w_exponents, need_dX, "w_codes", "dX")):
+        if codes is None and exponents is None:
+            if need:
+                raise ValueError(f"{name}: None, but {of} is asked for")
+        elif codes is None or exponents is None:
+            raise ValueError(f"{name}: codes and exponents go together")
+        elif name == "x_codes":
+            M = _image_of(codes, exponents, K, name)
+        else:
+            N = _image_of(codes, exponents, K, name)
     dev = dY.device
     _same_device(dev, x_codes=x_codes, w_codes=w_codes, bits=bits)
     if shape != [M, N]:
@@ -1128,8 +1139,8 @@ def _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponen
     nb = lib().phonlp_linear_e4m3_backward_ws_bytes(M, N, K, code)
     ws = _ws(nb, dev)
     ptr = lambda t: None if t is None else t.data_ptr()
-    _run(dev, "phonlp_linear_e4m3_backward", dY.data_ptr(), code, ld, ptr(bits), x_codes.data_ptr(), x_exponents.data_ptr(),
-         w_codes.data_ptr(), w_exponents.data_ptr(), M, N, K, ptr(dX), ptr(dW), ptr(db), ws.data_ptr(), max(nb, 256))
+    _run(dev, "phonlp_linear_e4m3_backward", dY.data_ptr(), code, ld, ptr(bits), ptr(x_codes), ptr(x_exponents), ptr(w_codes),
+         ptr(w_exponents), M, N, K, ptr(dX), ptr(dW), ptr(db), ws.data_ptr(), max(nb, 256))
     return dX, dW, db
 
 
@@ -1230,8 +1241,9 @@ def _(x_codes, x_exponents, w_codes, w_exponents, bias, K, relu, dtype, want_bit
 
 
 @torch.library.custom_op("phonlp_amd::linear_e4m3_backward", mutates_args=())
-def _linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x_exponents: Tensor, w_codes: Tensor, w_exponents: Tensor,
-                          K: int, need_dX: bool, need_dW: bool, need_db: bool) -> Tuple[Tensor, Tensor, Tensor]:
+def _linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Optional[Tensor], x_exponents: Optional[Tensor],
+                          w_codes: Optional[Tensor], w_exponents: Optional[Tensor], K: int, need_dX: bool, need_dW: bool,
+                          need_db: bool) -> Tuple[Tensor, Tensor, Tensor]:
     got = _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db)
     types = dY.dtype, torch.float32, torch.float32
     return tuple(dY.new_empty((0,), dtype=t) if g is None else g for g, t in zip(got, types))
@@ -1239,7 +1251,7 @@ def _linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Tensor, x
 
 @_linear_e4m3_backward.register_fake
 def _(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db):
-    M, N = x_codes.shape[0], w_codes.shape[0]
+    M, N = dY.shape
     return (dY.new_empty((M, K) if need_dX else (0,)), dY.new_empty((N, K) if need_dW else (0,), dtype=torch.float32),
             dY.new_empty((N,) if need_db else (0,), dtype=torch.float32))
 
