@@ -1108,19 +1108,21 @@ def linear_e4m3_backward(dY: Tensor, bits: Optional[Tensor], x_codes: Optional[T
     return _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db)
 
 
+def _operand_of(codes: Optional[Tensor], exponents: Optional[Tensor], K: int, name: str, rows: int, need: bool, of: str) -> int:
+    """_image_of of an operand that may be missing where its gradient is not asked for; -> its rows, or `rows` without it."""
+    if codes is not None and exponents is not None:
+        return _image_of(codes, exponents, K, name)
+    if codes is not exponents:
+        raise ValueError(f"{name}: codes and exponents go together")
+    if need:
+        raise ValueError(f"{name}: None, but {of} is asked for")
+    return rows
+
+
 def _linear_e4m3_backward_now(dY, bits, x_codes, x_exponents, w_codes, w_exponents, K, need_dX, need_dW, need_db):
     code, ld, *shape = _rows_of(dY, "dY")
-    M, N = shape
-    for codes, exponents, need, name, of in ((x_codes, x_exponents, need_dW, "x_codes", "dW"), (w_codes, w_exponents, need_dX, "w_codes", "dX")):
-        if codes is None and exponents is None:
-            if need:
-                raise ValueError(f"{name}: None, but {of} is asked for")
-        elif codes is None or exponents is None:
-            raise ValueError(f"{name}: codes and exponents go together")
-        elif name == "x_codes":
-            M = _image_of(codes, exponents, K, name)
-        else:
-            N = _image_of(codes, exponents, K, name)
+    M = _operand_of(x_codes, x_exponents, K, "x_codes", shape[0], need_dW, "dW")
+    N = _operand_of(w_codes, w_exponents, K, "w_codes", shape[1], need_dX, "dX")
     dev = dY.device
     _same_device(dev, x_codes=x_codes, w_codes=w_codes, bits=bits)
     if shape != [M, N]:
