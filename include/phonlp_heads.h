@@ -528,16 +528,16 @@ int phonlp_e4m3_values(const void *codes, const uint8_t *exponents, int rows, in
 
 /* Y[M,N] = act(X^ . W^^T + bias[N]) with X^, W^ the values of two images with the same K; fp32 sums, Y in `type`, row pitch N.
  * bias may be NULL.  relu: max(., 0), NaN kept.  bits: NULL, or [M, ceil(N / 32)] words with bit n % 32 of word n / 32 set where the
- * stored Y[m][n] > 0 (zero behind N) -- what the backward needs of a ReLU layer's output.  Products are exact, added in
- * fp32 and rounded to `type` once.  ceil(M / 128) * ceil(N / 128) < 2^23. */
+ * stored Y[m][n] > 0 (zero behind N) -- what the backward needs of a ReLU layer's output.  Products are exact (operands
+ * to multiples of 2^-133), added in fp32 and rounded to `type` once.  ceil(M / 128) * ceil(N / 128) < 2^23. */
 int phonlp_linear_e4m3(const void *x_codes, const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents,
                        const float *bias, void *y, int type, uint32_t *bits, int M, int N, int K, int relu, void *stream);
 
 /* Backward of that layer from its 8-bit checkpoint: dY [M,N] in `type` (row pitch lddy), bits as above (NULL: no ReLU), the images
  * of the layer's input and weight ->  dZ = dY where the bit is set, dX [M,K] = dZ . W^ in `type`, dW [N,K] = dZ^T . X^ and
  * db [N] = column sums of dZ in fp32.  Any of dX / dW / db may be NULL, x's image without dW and w's without dX too.  Products are
- * exact (dZ in up to three bf16 pieces), sums fp32 in a fixed order.  M <= 2^24, N and K <= 2^21; ceil(M / 128) * ceil(K / 128) and
- * ceil(N / 128) * ceil(K / 128) < 2^22. */
+ * exact (dZ in up to three bf16 pieces; operands to multiples of 2^-133), sums fp32 in a fixed order.  M <= 2^24, N and K <= 2^21;
+ * ceil(M / 128) * ceil(K / 128) and ceil(N / 128) * ceil(K / 128) < 2^22. */
 size_t phonlp_linear_e4m3_backward_ws_bytes(int M, int N, int K, int type);
 int phonlp_linear_e4m3_backward(const void *dy, int type, long lddy, const uint32_t *bits, const void *x_codes,
                                 const uint8_t *x_exponents, const void *w_codes, const uint8_t *w_exponents, int M, int N, int K,

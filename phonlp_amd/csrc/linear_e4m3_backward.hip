@@ -4,7 +4,7 @@
 // Products on v_mfma_f32_16x16x32_bf16 (2.05 PFLOP/s in a loop of nothing else, 32x32x16 1.84).  The values of an image are exact in bf16
 // (four significant bits, a power of two), and dZ is cut into bf16 pieces whose sum is dZ itself -- one for bf16, two for fp16 (11
 // bits), three for fp32 (24 bits), by truncation, so no piece can round past bf16's largest --, so every product is exact and only the
-// fp32 sums round.  (Values under 2^-126 may lose low bits.)
+// fp32 sums round.  (What an operand has below 2^-133, bf16's smallest step, is lost.)
 #include <type_traits>
 
 #include "e4m3.h"

@@ -1051,7 +1051,8 @@ def _e4m3_rows_now(x: Tensor) -> Tuple[Tensor, Tensor]:
 
 
 def e4m3_values(codes: Tensor, exponents: Tensor, K: int, dtype: torch.dtype = torch.float32) -> Tensor:
-    """The values [rows, K] that an e4m3 image stands for: exact in fp32 and bf16, 16-bit types saturate at their largest."""
+    """The values [rows, K] that an e4m3 image stands for: exact in fp32 and, down to its smallest
+    step 2^-133, in bf16; 16-bit types saturate at their largest."""
     return (torch.ops.phonlp_amd.e4m3_values if _traced(codes) else _e4m3_values_now)(codes, exponents, K, dtype)
 
 

@@ -52,3 +52,21 @@ def test_results_are_roundings_of_fp32_sums(dev, dtype, M, N, K):
     err = (y.double() - want) / want.square().mean().sqrt()
     limit = float(t.mean() / want.square().mean().sqrt()) + 8 * torch.finfo(dtype).eps / 2 / np.sqrt(err.numel())
     assert abs(float(err.mean())) <= limit
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 128), (300, 900, 200)])
+def test_operands_down_to_their_smallest_step(dev, dtype, M, N, K):
+    """x of up to fifteen steps of 2^-133, dY of up to fifteen (fp32: 4096), w and the kept input of whole numbers times 2^100: exact products and sums."""
+    from phonlp_amd import ops
+    g = torch.Generator(device=dev).manual_seed(M)
+    draw = lambda most, *s: torch.randint(-most, most + 1, s, generator=g, device=dev).double()
+    x, w, kept = draw(15, M, K), draw(3, N, K), draw(3, M, K)
+    dY = draw(2 ** 12 if dtype == torch.float32 else 15, M, N)
+    assert 2 ** 12 * 3 * max(M, N) < 2 ** 24
+    small, large = lambda t, kind: (t * 2.0 ** -133).to(kind), lambda t: ops.e4m3_rows((t * 2.0 ** 100).float())
+    wi = large(w)
+    y, _ = ops.linear_e4m3(*ops.e4m3_rows(small(x, dtype)), *wi, None, K, False, dtype)
+    assert torch.equal(y, ((x @ w.t()) * 2.0 ** -33).to(dtype))
+    dX, dW, _ = ops.linear_e4m3_backward(small(dY, dtype), None, *large(kept), *wi, K)
+    assert torch.equal(dX, ((dY @ w) * 2.0 ** -33).to(dtype)) and torch.equal(dW.double(), (dY.t() @ kept) * 2.0 ** -33)
