@@ -413,7 +413,8 @@ def pos_loss(heads, params, enc, sentlens, upos, ignore_index=1, masks=None, den
 
 
 def ner_loss(heads, params, enc, sentlens, tags, masks=None, dense=None):
-    """Differentiable `loss` of ref jointmodel/model.py:139-160 (ner_forward: CRF NLL averaged over the batch).  `masks`, `dense` as in parser_loss."""
+    """Differentiable `loss` of ref jointmodel/model.py:139-160 (ner_forward: CRF NLL averaged over the batch).
+    `masks`, `dense` as in parser_loss."""
     return _loss_node(lambda e: heads.ner_backward(e, sentlens, tags, masks, dense), enc, params)
 
 
@@ -480,7 +481,8 @@ class _LinearE4m3Fn(torch.autograd.Function):
 def linear_e4m3(x, weight, bias=None, relu=False):
     """Differentiable y = act(x @ weight.T + bias) with both operands in e4m3 (a power-of-two scale per row and block of 128 columns),
     fp32 sums, y of x's type: x [..., K], weight [N, K], bias [N] in fp32 / bf16 / fp16.  What it keeps for the backward are the 8-bit
-    images (x's where weight, weight's where x needs a gradient) and one bit per output of a ReLU; the quantisation counts as the identity.  Under torch.no_grad nothing is kept."""
+    images (x's where weight, weight's where x needs a gradient) and one bit per output of a ReLU; the quantisation counts as the
+    identity.  Under torch.no_grad nothing is kept."""
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:  # an image does not know where inside its last block K ends
         raise ValueError(f"weight: expected [N, K] with x's K columns, got {tuple(weight.shape)} for x {tuple(x.shape)}")
     return _LinearE4m3Fn.apply(x, weight, bias, bool(relu))

@@ -2,8 +2,8 @@
 //
 // Block of x: a = its largest finite magnitude, e = the smallest integer >= -126 with a <= 448 * 2^e, code = e4m3(x * 2^-e)
 // (nearest even).  A power of two, not a / 448: the scaling is then exact and the value code * 2^e is exact in fp32 and, from its
-// smallest step 2^-133 on, in bf16 (the conversion v_cvt_scalef32 applies it), while e4m3 is a floating-point code whose relative precision does not depend on where in
-// its range a block lies.
+// smallest step 2^-133 on, in bf16 (the conversion v_cvt_scalef32 applies it), while e4m3 is a floating-point code whose relative
+// precision does not depend on where in its range a block lies.
 //   codes     [rows][Kp]   Kp = K rounded up to 128, zero behind K (one block = one 128-byte line)
 //   exponents [rows][KB4]  e + 127 as a byte, KB4 = Kp / 128 rounded up to 4 (four blocks' exponents = one dword), 127 behind
 #pragma once

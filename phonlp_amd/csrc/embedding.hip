@@ -248,8 +248,8 @@ struct SumArgs {
 // fp32, 512 tokens 4.2 against 13.5; at worst, 512 times the same token of 1000 x 768 bf16, 30 against 15.
 constexpr int kFewMost = 512;
 template <int VEC, class T, class TO, class I>
-__global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld, const I *tokens, int N, int V, int E, long base, int rows, float scale,
-                                                            TO *table) {
+__global__ __launch_bounds__(256) void embedding_few_kernel(const T *d, long ld, const I *tokens, int N, int V, int E, long base, int rows,
+                                                            float scale, TO *table) {
     constexpr int UNROLL = 16;
     typedef typename Vec<T, VEC>::type Vt;
     __shared__ float shares[4][64 * VEC];

@@ -2,9 +2,9 @@
 //
 // Products on v_mfma_f32_16x16x32_bf16, whatever the result's type: the values of an image are exact in bf16, converted with their scale
 // from the codes as those leave LDS (v_cvt_scalef32_pk_bf16_fp8, two codes each), every product is exact and the sums are fp32
-// throughout (what an operand has below 2^-133, bf16's smallest step, is lost).  The 8-bit pipe, v_mfma_scale_f32_32x32x64_f8f6f4, would be up to twice as fast, but adds eight products at a time, each cut
-// off 13 bits below the largest of the eight (measured: 2^16 + 2^2 loses the small one): where large products cancel, what is left of
-// the result is lost, whatever its type.
+// throughout (what an operand has below 2^-133, bf16's smallest step, is lost).  The 8-bit pipe, v_mfma_scale_f32_32x32x64_f8f6f4, would
+// be up to twice as fast, but adds eight products at a time, each cut off 13 bits below the largest of the eight (measured: 2^16 + 2^2
+// loses the small one): where large products cancel, what is left of the result is lost, whatever its type.
 // Both operands are K-contiguous and an instruction's K order is free (A and B share it).
 #include <type_traits>
 

@@ -495,8 +495,7 @@ class TaskHeads:
         gh, gr = with_root(gold_head), with_root(gold_rel)
         live = (torch.arange(L, device=dev)[None, :] < lens[:, None]).reshape(M, 1)
         x = enc.reshape(M, E).contiguous()
-        pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_dep, bl(masks["wd_pos"]), f32(masks["drop_pos"]).reshape(M, -1),
-                                                       e4m3)
+        pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_dep, bl(masks["wd_pos"]), f32(masks["drop_pos"]).reshape(M, -1), e4m3)
         feat = torch.cat([x, pos_emb], 1).contiguous()
         m_wd = bl(masks["wd"])
         featd = TaskHeads._word_drop(feat, m_wd, w.repl_dep)
@@ -618,8 +617,7 @@ class TaskHeads:
             live = (torch.arange(L, device=dev)[None, :] < lens[:, None]).reshape(M, 1)
             x = enc.reshape(M, E).contiguous()
             pos_emb, _, pos_bw = TaskHeads._soft_pos_train(w, x, w.emb_ner, bl(masks["wd_pos"]),
-                                                           torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1),
-                                                           e4m3)
+                                                           torch.as_tensor(masks["drop_pos"]).to(dev, torch.float32).reshape(M, -1), e4m3)
             m_wd = bl(masks["wd"])
             featd = TaskHeads._word_drop(torch.cat([x, pos_emb], 1).contiguous(), m_wd, w.repl_ner)
             logits2 = (ops.linear(featd, w.ner_w, w.ner_b, True, None, 0) * live).contiguous()
